@@ -1,4 +1,5 @@
-"""ctypes binding of libh3vae_b200.so (the C ABI declared in include/h3vae_b200.h).
+"""ctypes binding of libh3vae_b200.so (the C ABI declared in include/h3vae_b200.h and
+include/h3vae_b200_kv.h).
 
 The shared library is the only compute path.  There is deliberately no CPU or
 PyTorch fallback: if the library is missing or a call fails, an exception is
@@ -85,7 +86,32 @@ _SIGNATURES = {
     "h3b_blend_accumulate": (c_int, [c_void_p, c_int, _i64p, _i64p, c_void_p, c_void_p, _i64p, c_void_p]),
 }
 
-EXPORTED_SYMBOLS = tuple(name for name in _SIGNATURES)
+
+
+class KvCacheStruct(ctypes.Structure):
+    """h3b_kv_cache of include/h3vae_b200_kv.h."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("k_sum", c_void_p),
+                ("num_pages", c_int64), ("kv_heads", c_int64), ("page_size", c_int64), ("head_dim", c_int64)]
+
+
+_kvp = POINTER(KvCacheStruct)
+
+# include/h3vae_b200_kv.h: the paged INT8 key/value cache
+_KV_SIGNATURES = {
+    "h3b_kv_write_i8": (c_int, [_kvp, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, _i64p, c_void_p, _i64p,
+                                c_int64, c_int, c_void_p]),
+    "h3b_kv_read_i8": (c_int, [_kvp, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,
+                               c_void_p]),
+    "h3b_attention_kv_i8_workspace_size": (c_size_t, [c_int64] * 8),
+    "h3b_attention_kv_i8": (c_int, [c_void_p, _i64p, _kvp, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64,
+                                    c_int64, c_float, c_int, c_int64, c_void_p, c_int64, c_int, c_void_p, _i64p,
+                                    c_void_p, c_void_p, c_size_t, c_void_p]),
+    "h3b_kv_select_i8_workspace_size": (c_size_t, [c_int64] * 4),
+    "h3b_kv_select_i8": (c_int, [c_void_p, _i64p, _kvp, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64,
+                                 c_int64, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
+}
+
+EXPORTED_SYMBOLS = tuple(_SIGNATURES) + tuple(_KV_SIGNATURES)
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
@@ -108,7 +134,7 @@ def load() -> ctypes.CDLL:
                 f"h3vae_b200 CUDA library not found at {LIB_PATH}; build it with "
                 "`python -c 'import __graft_entry__ as g; g.build()'` (no CPU fallback exists)")
         lib = ctypes.CDLL(str(LIB_PATH))
-        for name, (restype, argtypes) in _SIGNATURES.items():
+        for name, (restype, argtypes) in (*_SIGNATURES.items(), *_KV_SIGNATURES.items()):
             fn = getattr(lib, name)
             fn.restype = restype
             fn.argtypes = argtypes
@@ -134,6 +160,9 @@ def check(rc: int) -> None:
 def i64_array(values) -> ctypes.Array:
     vals = [int(v) for v in values]
     return (c_int64 * len(vals))(*vals)
+
+
+i64_x3 = c_int64 * 3
 
 
 def device_error(clear: bool = True) -> int:

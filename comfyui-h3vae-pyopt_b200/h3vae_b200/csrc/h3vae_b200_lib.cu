@@ -7,3 +7,6 @@
 #include "attention_tc.cu"
 #include "conv_in.cu"
 #include "conv_rgb.cu"
+#include "kv_cache.cu"
+#include "attention_kv.cu"
+#include "kv_select.cu"

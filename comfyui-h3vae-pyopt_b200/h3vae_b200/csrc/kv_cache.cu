@@ -1,0 +1,266 @@
+// Writing and reading the paged INT8 key/value cache.
+//
+// Write.  For the new tokens x of one (page, head) and K or V:
+//   a = max|x|;  s = max(a * fp32(1/127), 1e-30), and max(s, old scale) when the
+//   page keeps earlier tokens, whose codes become rint(code * (old / s)) if s
+//   grew;  code = rint(x * (1/s)).
+// One CTA per (page slot, head, K or V): the page's new values (at most 16 KB
+// of fp16) stay in registers between the maximum and the quantisation, so every
+// input is read once and every code written once.  Bound: HBM, 2 B read and
+// 1 B written per element.
+#include "kv_common.cuh"
+
+namespace h3b {
+
+constexpr int kKvThreads = 128;
+
+struct KvWriteParams {
+  KvView c;
+  const int32_t* start;
+  const int32_t* counts;
+  const void* x[2];        // K, V
+  int64_t stride[2][3];    // elements: batch, head, token
+  int tokens, dim;
+  bool vec[2];             // rows can be read 16 bytes at a time
+};
+
+// VPT: vectors of 8 elements per thread = page * dim / 1024.
+template <typename T, int VPT>
+__global__ void __launch_bounds__(kKvThreads) kv_write_kernel(const KvWriteParams p) {
+  __shared__ float s_max[kKvThreads / 32];
+  __shared__ int s_sum[kKvThreads / 32][128];
+  const int kv = blockIdx.x & 1, head = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const int count = p.counts ? min(p.counts[b], p.tokens) : p.tokens;
+  const int start = p.start[b];
+  if (start < 0) {
+    if (tid == 0 && count > 0) record_error(kErrKvPage);
+    return;
+  }
+  const int slot = (start >> p.c.page_shift) + (blockIdx.x >> 1);
+  const int64_t page_begin = static_cast<int64_t>(slot) << p.c.page_shift;
+  const int64_t end = static_cast<int64_t>(start) + count;
+  const int lo = static_cast<int>(max(static_cast<int64_t>(start), page_begin) - page_begin);   // first new row
+  const int hi = static_cast<int>(min(end - page_begin, static_cast<int64_t>(p.c.page)));       // past the last one
+  if (hi <= lo) return;
+  const int page = kv_page(p.c, b, slot);
+  if (page < 0) return;
+
+  const int chunks = p.dim >> 3;
+  const int64_t ph = static_cast<int64_t>(page) * p.c.heads + head;
+  int8_t* codes = p.c.code[kv] + ph * p.c.page * p.dim;
+  float* scale_at = p.c.scale[kv] + ph;
+  const T* src = static_cast<const T*>(p.x[kv]) + b * p.stride[kv][0] + head * p.stride[kv][1];
+  const int64_t row0 = page_begin - start;   // token of the page's row 0
+  const float old_scale = *scale_at;
+
+  // the new rows, and the largest magnitude among them (NaN and infinities give NaN or +inf)
+  float x[VPT][8];
+  float top = 0.0f;
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int i = tid + j * kKvThreads, row = i / chunks, col = (i % chunks) * 8;
+    if (row >= lo && row < hi) {
+      load8(src + (row0 + row) * p.stride[kv][2] + col, p.vec[kv], x[j]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        top = fmaxf(top, fabsf(x[j][e]));
+        bad |= !(fabsf(x[j][e]) <= 3.4028235e38f);
+      }
+    }
+  }
+  if (bad) top = INFINITY;
+  top = warp_max(top);
+  if ((tid & 31) == 0) s_max[tid >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kKvThreads / 32; ++w) top = fmaxf(top, s_max[w]);
+
+  float s = fmaxf(__fmul_rn(top, kKvInv127), kKvMinScale);
+  if (lo > 0) s = old_scale > s ? old_scale : s;
+  const bool lost = top == INFINITY || (lo > 0 && isnan(old_scale));
+  const bool grown = lo > 0 && s > old_scale;
+  const bool complete = kv == 0 && hi == p.c.page;
+  const float inv = __frcp_rn(s), ratio = __fdiv_rn(old_scale, s);
+  int sum[8] = {};
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int i = tid + j * kKvThreads, row = i / chunks, col = (i % chunks) * 8;
+    uint2* at = reinterpret_cast<uint2*>(codes + row * p.dim + col);
+    uint2 w = make_uint2(0u, 0u);
+    bool store = false;
+    if (row >= lo && row < hi) {
+      store = true;
+      if (!lost) {   // |x * inv| <= 127 * (1 + 2^-22): no clamp is needed after rounding
+        uint32_t q[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = rint_bits(__fmul_rn(x[j][e], inv));
+        w = make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+      }
+    } else if (row < lo && (grown || complete)) {
+      w = *at;
+      if (grown && !lost) {
+        store = true;
+        float f[8];
+        codes_to_f32(w.x, f);
+        codes_to_f32(w.y, f + 4);
+        uint32_t q[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = rint_bits(__fmul_rn(f[e], ratio));
+        w = make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+      }
+    }
+    if (store) *at = w;
+    if (complete) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] += static_cast<int8_t>((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
+    }
+  }
+  if (tid == 0) *scale_at = lost ? __int_as_float(0x7fffffff) : s;
+  if (complete) {
+    // a thread's vectors share their column (kKvThreads is a multiple of `chunks`)
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      for (int o = chunks; o < 32; o <<= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
+    if ((tid & 31) < chunks) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s_sum[tid >> 5][(tid & 31) * 8 + e] = sum[e];
+    }
+    __syncthreads();
+    if (tid < p.dim) {
+      int t = 0;
+#pragma unroll
+      for (int w = 0; w < kKvThreads / 32; ++w) t += s_sum[w][tid];
+      p.c.k_sum[ph * p.dim + tid] = static_cast<int16_t>(t);
+    }
+  }
+}
+
+// Read: one thread per 8 codes of K and of V (8 B in, 16 B out of fp16 each).
+struct KvReadParams {
+  KvView c;
+  const int32_t* start;
+  const int32_t* lengths;
+  void* out[2];
+  int tokens, chunk_shift;   // dim = 8 << chunk_shift
+};
+
+constexpr int kKvReadThreads = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(kKvReadThreads) kv_read_kernel(const KvReadParams p) {
+  const int head = blockIdx.y, b = blockIdx.z;
+  const int i = blockIdx.x * kKvReadThreads + threadIdx.x;
+  const int row = i >> p.chunk_shift, col = (i & ((1 << p.chunk_shift) - 1)) * 8;
+  if (row >= p.tokens) return;
+  const int dim = 8 << p.chunk_shift;
+  const int64_t pos = static_cast<int64_t>(p.start ? p.start[b] : 0) + row;
+  int page = -1;
+  if (pos >= 0 && pos < p.lengths[b]) page = kv_page(p.c, b, static_cast<int>(pos >> p.c.page_shift));
+  const int64_t ph = static_cast<int64_t>(page) * p.c.heads + head;
+  const int64_t from = (ph * p.c.page + (pos & (p.c.page - 1))) * dim + col;
+  const int64_t to = ((static_cast<int64_t>(b) * p.c.heads + head) * p.tokens + row) * dim + col;
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    float x[8] = {};
+    if (page >= 0) {
+      const uint2 w = *reinterpret_cast<const uint2*>(p.c.code[kv] + from);
+      const float s = p.c.scale[kv][ph];
+      codes_to_f32(w.x, x);
+      codes_to_f32(w.y, x + 4);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(x[e], s);
+    }
+    __align__(16) T y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) from_f32(x[e], y[e]);
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out[kv]) + to);
+#pragma unroll
+    for (int k = 0; k < KvVec8<T>::kWords / 4; ++k) dst[k] = reinterpret_cast<const uint4*>(y)[k];
+  }
+}
+
+}  // namespace h3b
+
+namespace {
+
+template <typename T>
+void launch_kv_write(const h3b::KvWriteParams& p, dim3 grid, cudaStream_t st) {
+  switch (p.c.page * p.dim / 1024) {
+    case 1: h3b::kv_write_kernel<T, 1><<<grid, h3b::kKvThreads, 0, st>>>(p); break;
+    case 2: h3b::kv_write_kernel<T, 2><<<grid, h3b::kKvThreads, 0, st>>>(p); break;
+    case 4: h3b::kv_write_kernel<T, 4><<<grid, h3b::kKvThreads, 0, st>>>(p); break;
+    case 8: h3b::kv_write_kernel<T, 8><<<grid, h3b::kKvThreads, 0, st>>>(p); break;
+    default: h3b::kv_write_kernel<T, 16><<<grid, h3b::kKvThreads, 0, st>>>(p); break;
+  }
+}
+
+}  // namespace
+
+extern "C" int h3b_kv_write_i8(const h3b_kv_cache* cache, const int32_t* page_table, int64_t batch,
+                               int64_t table_width, const int32_t* start, const int32_t* counts, const void* k,
+                               const int64_t* k_strides, const void* v, const int64_t* v_strides, int64_t tokens,
+                               int dtype, h3b_stream_t stream) {
+  const char* name = "h3b_kv_write_i8";
+  h3b::KvWriteParams p{};
+  int rc = h3b_host::kv_view(name, cache, page_table, batch, table_width, &p.c);
+  if (rc) return rc;
+  if (!start || !k || !v || !k_strides || !v_strides) return h3b_host::set_error(H3B_EINVAL, "%s: NULL argument", name);
+  if (dtype != H3B_TYPE_F16 && dtype != H3B_TYPE_BF16 && dtype != H3B_TYPE_F32)
+    return h3b_host::set_error(H3B_EINVAL, "%s: unknown dtype %d", name, dtype);
+  if (tokens < 0 || tokens > (int64_t(1) << 30)) return h3b_host::set_error(H3B_EINVAL, "%s: bad token count", name);
+  if (tokens == 0) return H3B_OK;
+  p.start = start;
+  p.counts = counts;
+  p.x[0] = k;
+  p.x[1] = v;
+  p.tokens = (int)tokens;
+  p.dim = (int)cache->head_dim;
+  const int size = dtype == H3B_TYPE_F32 ? 4 : 2;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t* s = i ? v_strides : k_strides;
+    p.vec[i] = h3b_host::aligned16(p.x[i]);
+    for (int j = 0; j < 3; ++j) {
+      p.stride[i][j] = s[j];
+      p.vec[i] = p.vec[i] && s[j] * size % 16 == 0;
+    }
+  }
+  const int64_t slots = (tokens + p.c.page - 2) / p.c.page + 1;
+  if (slots > (int64_t(1) << 30) || cache->kv_heads > 65535)
+    return h3b_host::set_error(H3B_EUNSUPPORTED, "%s: problem too large", name);
+  dim3 grid((unsigned)(2 * slots), (unsigned)cache->kv_heads, (unsigned)batch);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == H3B_TYPE_F16) launch_kv_write<__half>(p, grid, st);
+  else if (dtype == H3B_TYPE_BF16) launch_kv_write<__nv_bfloat16>(p, grid, st);
+  else launch_kv_write<float>(p, grid, st);
+  return h3b_host::check_launch(name);
+}
+
+extern "C" int h3b_kv_read_i8(const h3b_kv_cache* cache, const int32_t* page_table, int64_t batch,
+                              int64_t table_width, const int32_t* start, const int32_t* lengths, void* k, void* v,
+                              int64_t tokens, int dtype, h3b_stream_t stream) {
+  const char* name = "h3b_kv_read_i8";
+  h3b::KvReadParams p{};
+  int rc = h3b_host::kv_view(name, cache, page_table, batch, table_width, &p.c);
+  if (rc) return rc;
+  if (!lengths || !k || !v) return h3b_host::set_error(H3B_EINVAL, "%s: NULL argument", name);
+  if (!h3b_host::aligned16(k) || !h3b_host::aligned16(v))
+    return h3b_host::set_error(H3B_EINVAL, "%s: outputs must be 16-byte aligned", name);
+  if (tokens < 0 || tokens > (int64_t(1) << 26)) return h3b_host::set_error(H3B_EINVAL, "%s: bad token count", name);
+  if (tokens == 0) return H3B_OK;
+  p.start = start;
+  p.lengths = lengths;
+  p.out[0] = k;
+  p.out[1] = v;
+  p.tokens = (int)tokens;
+  p.chunk_shift = cache->head_dim == 64 ? 3 : 4;
+  const int64_t vecs = tokens << p.chunk_shift;
+  dim3 grid((unsigned)((vecs + h3b::kKvReadThreads - 1) / h3b::kKvReadThreads), (unsigned)cache->kv_heads,
+            (unsigned)batch);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == H3B_TYPE_F16) h3b::kv_read_kernel<__half><<<grid, h3b::kKvReadThreads, 0, st>>>(p);
+  else if (dtype == H3B_TYPE_BF16) h3b::kv_read_kernel<__nv_bfloat16><<<grid, h3b::kKvReadThreads, 0, st>>>(p);
+  else if (dtype == H3B_TYPE_F32) h3b::kv_read_kernel<float><<<grid, h3b::kKvReadThreads, 0, st>>>(p);
+  else return h3b_host::set_error(H3B_EINVAL, "%s: unknown dtype %d", name, dtype);
+  return h3b_host::check_launch(name);
+}

@@ -1,0 +1,233 @@
+// Page selection for sparse attention over the paged INT8 cache.
+//
+// A row (query token, kv head) scores every complete page before its own with
+//   max over the group's heads of float(q8 . k_sum[page]) * s_q, times k_scale[page]
+// (q8, s_q: the row quantisation of the query; k_sum: the sum of the page's K
+// codes, so the score is the query's mean product with the page's keys up to a
+// common factor) and keeps the best n - 1 and its own page.  The products are
+// whole numbers below 2^31, so scores do not depend on the summation order and
+// ties (lower page first) are exact.
+//
+// Two kernels: scores (a thread per page, all rows of the sequence and head
+// from shared memory) and the selection (a block per row: a radix select of the
+// (n-1)-th largest key, then an ordered compaction).
+#include "kv_common.cuh"
+
+namespace h3b {
+
+struct KvSelectParams {
+  KvView c;
+  const void* q;
+  const int32_t* lengths;
+  const int32_t* counts;
+  uint32_t* keys;        // [batch, heads, tokens, width]
+  int32_t* selected;
+  int64_t qs[3];
+  int group, tokens, n;
+};
+
+// Last page ordinal row t of sequence b sees, -1 if none.
+__device__ __forceinline__ int kv_last_page(const KvSelectParams& p, int b, int t) {
+  int len = max(p.lengths[b], 0);
+  if (len > p.c.width * p.c.page) {
+    record_error(kErrKvPage);
+    len = p.c.width * p.c.page;
+  }
+  const int n = p.counts ? min(p.counts[b], p.tokens) : p.tokens;
+  const int pos = len - n + t;
+  return t >= n || pos < 0 ? -1 : pos >> p.c.page_shift;
+}
+
+constexpr int kSelThreads = 256;
+constexpr int kSelRows = 64;     // query rows held in shared memory at once
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kSelThreads) kv_score_kernel(const KvSelectParams p) {
+  __shared__ __align__(16) uint32_t s_q[kSelRows][D / 4];   // four codes a word
+  __shared__ float s_s[kSelRows];
+  const int head = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int slot = blockIdx.x * kSelThreads + threadIdx.x;
+  const int last = kv_last_page(p, b, (p.counts ? min(p.counts[b], p.tokens) : p.tokens) - 1);
+  if (static_cast<int>(blockIdx.x) * kSelThreads >= last) return;   // no complete page here (uniform)
+  uint32_t k[D / 2];
+  float k_scale = 0.0f;
+  const int page = slot < last ? kv_page(p.c, b, slot) : -1;
+  if (page >= 0) {
+    const int64_t ph = static_cast<int64_t>(page) * p.c.heads + head;
+    k_scale = p.c.scale[0][ph];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      const uint4 w = *reinterpret_cast<const uint4*>(p.c.k_sum + ph * D + 8 * i);
+      k[4 * i] = w.x, k[4 * i + 1] = w.y, k[4 * i + 2] = w.z, k[4 * i + 3] = w.w;
+    }
+  }
+  const int per = max(1, kSelRows / p.group);      // query tokens per round
+  float best = 0.0f;
+  for (int t0 = 0; t0 < p.tokens; t0 += per) {
+    const int t1 = min(t0 + per, p.tokens);
+    for (int g0 = 0; g0 < p.group; g0 += kSelRows) {   // groups wider than the buffer take several rounds
+      const int g1 = min(g0 + kSelRows, p.group), gn = g1 - g0, rows = (t1 - t0) * gn;
+      __syncthreads();
+      for (int r = warp; r < rows; r += kSelThreads / 32) {
+        const int t = t0 + r / gn, h = head * p.group + g0 + r % gn;
+        const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1] + t * p.qs[2];
+        float x[D / 32], top = 0.0f;
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {
+          x[e] = to_f32(q[lane * (D / 32) + e]);
+          top = fmaxf(top, fabsf(x[e]));
+        }
+        const float s = fmaxf(__fmul_rn(warp_max(top), kKvInv127), kKvMinScale), inv = __frcp_rn(s);
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e)
+          reinterpret_cast<uint8_t*>(s_q[r])[lane * (D / 32) + e] = static_cast<uint8_t>(rint_bits(__fmul_rn(x[e], inv)));
+        if (lane == 0) s_s[r] = s;
+      }
+      __syncthreads();
+      if (page >= 0) {
+        for (int r = 0; r < rows; ++r) {
+          int dot = 0;
+#pragma unroll
+          for (int i = 0; i < D / 4; ++i) {
+            const int w = static_cast<int>(s_q[r][i]);
+            dot = __dp2a_lo(static_cast<int>(k[2 * i]), w, dot);
+            dot = __dp2a_hi(static_cast<int>(k[2 * i + 1]), w, dot);
+          }
+          const float x = __fmul_rn(static_cast<float>(dot), s_s[r]);
+          const int g = r % gn;
+          best = g0 + g == 0 ? x : fmaxf(best, x);
+          if (g0 + g + 1 == p.group) {
+            const float y = __fadd_rn(__fmul_rn(best, k_scale), 0.0f);   // -0 becomes +0
+            const uint32_t key = isnan(y) ? 0xffffffffu : float_to_ordered(y);
+            const int64_t row = (static_cast<int64_t>(b) * p.c.heads + head) * p.tokens + t0 + r / gn;
+            p.keys[row * p.c.width + slot] = key;
+          }
+        }
+      } else if (slot < last && g1 == p.group) {   // a bad page number: never worth choosing
+        for (int t = t0; t < t1; ++t)
+          p.keys[((static_cast<int64_t>(b) * p.c.heads + head) * p.tokens + t) * p.c.width + slot] = 0u;
+      }
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kSelThreads) kv_pick_kernel(const KvSelectParams p) {
+  __shared__ int s_hist[256];
+  __shared__ int s_scan[kSelThreads / 32][2];
+  __shared__ int s_pick[2];
+  const int t = blockIdx.x, head = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t row = (static_cast<int64_t>(b) * p.c.heads + head) * p.tokens + t;
+  int32_t* out = p.selected + row * p.n;
+  const uint32_t* keys = p.keys + row * p.c.width;
+  const int last = kv_last_page(p, b, t);
+  if (last < p.n) {   // every page fits
+    for (int i = tid; i < p.n; i += kSelThreads) out[i] = i <= last ? i : -1;
+    return;
+  }
+  const int want = p.n - 1;
+  if (want == 0) {
+    if (tid == 0) out[0] = last;
+    return;
+  }
+  // radix select: the want-th largest key, 8 bits a pass
+  uint32_t prefix = 0, mask = 0;
+  int left = want;
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    s_hist[tid] = 0;
+    __syncthreads();
+    for (int i = tid; i < last; i += kSelThreads) {
+      const uint32_t k = keys[i];
+      if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & 255u], 1);
+    }
+    __syncthreads();
+    if (tid == 0) {
+      int above = 0, d = 255;
+      while (d > 0 && above + s_hist[d] < left) above += s_hist[d--];
+      s_pick[0] = d;
+      s_pick[1] = left - above;
+    }
+    __syncthreads();
+    prefix |= static_cast<uint32_t>(s_pick[0]) << shift;
+    mask |= 255u << shift;
+    left = s_pick[1];
+  }
+  // keys above the threshold, and the first `left` that equal it, in page order
+  int n_out = 0, n_tie = 0;
+  for (int i0 = 0; i0 < last; i0 += kSelThreads) {
+    const int i = i0 + tid;
+    const uint32_t k = i < last ? keys[i] : 0u;
+    const bool tie = i < last && k == prefix, above = i < last && k > prefix;
+    const unsigned mt = __ballot_sync(0xffffffffu, tie), ma = __ballot_sync(0xffffffffu, above);
+    if (lane == 0) {
+      s_scan[warp][0] = __popc(mt);
+      s_scan[warp][1] = __popc(ma);
+    }
+    __syncthreads();
+    int ties = n_tie, aboves = 0, all_t = 0, all_a = 0;
+    for (int w = 0; w < kSelThreads / 32; ++w) {
+      if (w < warp) ties += s_scan[w][0], aboves += s_scan[w][1];
+      all_t += s_scan[w][0];
+      all_a += s_scan[w][1];
+    }
+    ties += __popc(mt & ((1u << lane) - 1u));        // ties before this page
+    aboves += __popc(ma & ((1u << lane) - 1u));
+    if (above || (tie && ties < left)) out[n_out + aboves + min(ties, left) - min(n_tie, left)] = i;
+    n_out += all_a + min(n_tie + all_t, left) - min(n_tie, left);
+    n_tie += all_t;
+    __syncthreads();
+  }
+  if (tid == 0) out[want] = last;
+}
+
+}  // namespace h3b
+
+extern "C" size_t h3b_kv_select_i8_workspace_size(int64_t batch, int64_t kv_heads, int64_t tokens,
+                                                  int64_t table_width) {
+  if (batch <= 0 || kv_heads <= 0 || tokens <= 0 || table_width <= 0) return 16;
+  return ((size_t)batch * kv_heads * tokens * table_width * 4 + 15) & ~size_t(15);
+}
+
+extern "C" int h3b_kv_select_i8(const void* q, const int64_t* q_strides, const h3b_kv_cache* cache,
+                                const int32_t* page_table, int64_t batch, int64_t table_width, const int32_t* lengths,
+                                const int32_t* counts, int64_t q_heads, int64_t tokens, int64_t n_selected, int dtype,
+                                int32_t* selected, void* workspace, size_t workspace_bytes, h3b_stream_t stream) {
+  const char* name = "h3b_kv_select_i8";
+  h3b::KvSelectParams p{};
+  int rc = h3b_host::kv_view(name, cache, page_table, batch, table_width, &p.c);
+  if (rc) return rc;
+  if (!q || !q_strides || !lengths || !selected) return h3b_host::set_error(H3B_EINVAL, "%s: NULL argument", name);
+  if (dtype != H3B_TYPE_F16 && dtype != H3B_TYPE_BF16)
+    return h3b_host::set_error(H3B_EINVAL, "%s: q must be fp16 or bf16", name);
+  if (q_heads <= 0 || q_heads % cache->kv_heads || q_heads > 65535)
+    return h3b_host::set_error(H3B_EINVAL, "%s: q_heads must be a positive multiple of kv_heads", name);
+  if (tokens < 0 || tokens > (int64_t(1) << 20) || n_selected <= 0 || n_selected > (int64_t(1) << 20))
+    return h3b_host::set_error(H3B_EINVAL, "%s: bad token count or page count", name);
+  if (tokens == 0) return H3B_OK;
+  if (!workspace || !h3b_host::aligned16(workspace) ||
+      workspace_bytes < h3b_kv_select_i8_workspace_size(batch, cache->kv_heads, tokens, table_width))
+    return h3b_host::set_error(H3B_EINVAL, "%s: workspace missing, misaligned or too small", name);
+  p.q = q;
+  p.lengths = lengths;
+  p.counts = counts;
+  p.keys = static_cast<uint32_t*>(workspace);
+  p.selected = selected;
+  for (int i = 0; i < 3; ++i) p.qs[i] = q_strides[i];
+  p.group = (int)(q_heads / cache->kv_heads);
+  p.tokens = (int)tokens;
+  p.n = (int)n_selected;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  dim3 g1((unsigned)((table_width + h3b::kSelThreads - 1) / h3b::kSelThreads), (unsigned)cache->kv_heads, (unsigned)batch);
+  dim3 g2((unsigned)tokens, (unsigned)cache->kv_heads, (unsigned)batch);
+  const bool wide = cache->head_dim == 128;
+  if (dtype == H3B_TYPE_F16) {
+    if (wide) h3b::kv_score_kernel<__half, 128><<<g1, h3b::kSelThreads, 0, st>>>(p);
+    else h3b::kv_score_kernel<__half, 64><<<g1, h3b::kSelThreads, 0, st>>>(p);
+  } else {
+    if (wide) h3b::kv_score_kernel<__nv_bfloat16, 128><<<g1, h3b::kSelThreads, 0, st>>>(p);
+    else h3b::kv_score_kernel<__nv_bfloat16, 64><<<g1, h3b::kSelThreads, 0, st>>>(p);
+  }
+  rc = h3b_host::check_launch(name);
+  if (rc) return rc;
+  h3b::kv_pick_kernel<<<g2, h3b::kSelThreads, 0, st>>>(p);
+  return h3b_host::check_launch(name);
+}

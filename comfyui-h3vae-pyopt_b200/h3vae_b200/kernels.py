@@ -739,3 +739,157 @@ def attention_f16(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: floa
                                              float(scale), _stream(dev)))
     _count(1)
     return out
+
+
+# ---------------------------------------------------------------------------
+# Paged INT8 key/value cache (h3vae_b200.kv_cache.KVCacheI8)
+# ---------------------------------------------------------------------------
+_KV_TYPES = {F16: 0, torch.bfloat16: 1, F32: 2}
+_I32 = torch.int32
+
+
+def _kv_index(t: torch.Tensor | None, name: str, shape: tuple, dev: torch.device) -> int | None:
+    """Data pointer of a contiguous int32 tensor of `shape` on `dev` (None passes)."""
+    if t is None:
+        return None
+    if t.dtype != _I32 or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+    if t.device != dev:
+        raise ValueError(f"{name} must be on the cache's device")
+    return t.data_ptr()
+
+
+def _kv_table(cache, page_table: torch.Tensor) -> tuple[int, int, int]:
+    if page_table.ndim != 2:
+        raise ValueError("page_table must be int32 [batch, pages]")
+    batch, width = page_table.shape
+    return _kv_index(page_table, "page_table", (batch, width), cache.device), batch, width
+
+
+def _kv_rows(t: torch.Tensor, name: str, types: tuple, cache) -> None:
+    if t.device != cache.device:
+        raise ValueError(f"{name} must be on the cache's device")
+    if t.ndim != 4 or t.dtype not in types or t.shape[3] != cache.head_dim or (t.stride(3) != 1 and t.numel()):
+        raise ValueError(f"{name} must be [batch, heads, tokens, {cache.head_dim}] with unit dim stride, one of {types}")
+
+
+def _strides3(t: torch.Tensor):
+    s = t.stride()
+    return _lib.i64_x3(s[0], s[1], s[2])
+
+
+def kv_write_i8(cache, page_table: torch.Tensor, start: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
+                counts: torch.Tensor | None = None) -> None:
+    """Quantise k, v [B, H, T, D] (fp16, bf16 or fp32, any strides with unit dim stride) into tokens start[b] ..
+    start[b] + counts[b] - 1 (counts None: T) of each sequence's pages, in place.  One scale per (page, head);
+    a page that already holds earlier tokens keeps the larger scale and requantises them when it grew.
+    page_table int32 [B, pages], start and counts int32 [B]."""
+    table, batch, width = _kv_table(cache, page_table)
+    _kv_rows(k, "k", (F16, torch.bfloat16, F32), cache)
+    _kv_rows(v, "v", (k.dtype,), cache)
+    if k.shape != v.shape or k.shape[0] != batch or k.shape[1] != cache.kv_heads:
+        raise ValueError(f"k and v must both be [{batch}, {cache.kv_heads}, tokens, {cache.head_dim}]")
+    if start is None:
+        raise ValueError("start must be int32 [batch]")
+    dev = cache.device
+    if not k.shape[2]:
+        return
+    _lib.check(_lib.load().h3b_kv_write_i8(
+        cache.struct, table, batch, width, _kv_index(start, "start", (batch,), dev),
+        _kv_index(counts, "counts", (batch,), dev), k.data_ptr(), _strides3(k), v.data_ptr(), _strides3(v), k.shape[2],
+        _KV_TYPES[k.dtype], _stream(dev)))
+    _count(1)
+
+
+def kv_read_i8(cache, page_table: torch.Tensor, lengths: torch.Tensor, tokens: int, *,
+               start: torch.Tensor | None = None, dtype: torch.dtype = F16) -> tuple[torch.Tensor, torch.Tensor]:
+    """Tokens start[b] .. start[b] + tokens - 1 (start None: from 0) as dense k, v [B, H, tokens, D] of `dtype`
+    (fp16, bf16 or fp32): code * scale, rounded once; zero at and past lengths[b]."""
+    table, batch, width = _kv_table(cache, page_table)
+    dev = cache.device
+    if dtype not in _KV_TYPES:
+        raise ValueError("dtype must be fp16, bf16 or fp32")
+    if lengths is None or tokens < 0:
+        raise ValueError("lengths must be int32 [batch] and tokens at least 0")
+    k = torch.empty((batch, cache.kv_heads, tokens, cache.head_dim), device=dev, dtype=dtype)
+    v = torch.empty_like(k)
+    if tokens:
+        _lib.check(_lib.load().h3b_kv_read_i8(
+            cache.struct, table, batch, width, _kv_index(start, "start", (batch,), dev),
+            _kv_index(lengths, "lengths", (batch,), dev), k.data_ptr(), v.data_ptr(), tokens, _KV_TYPES[dtype],
+            _stream(dev)))
+        _count(1)
+    return k, v
+
+
+def _kv_query(q: torch.Tensor, cache, batch: int) -> tuple[int, int]:
+    _kv_rows(q, "q", (F16, torch.bfloat16), cache)
+    if q.shape[0] != batch or q.shape[1] == 0 or q.shape[1] % cache.kv_heads:
+        raise ValueError(f"q must be [{batch}, a multiple of {cache.kv_heads} heads, tokens, {cache.head_dim}]")
+    return q.shape[1], q.shape[2]
+
+
+def attention_kv_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.Tensor, scale: float, *,
+                    counts: torch.Tensor | None = None, causal: bool = True, window: int = 0,
+                    selected: torch.Tensor | None = None, out: torch.Tensor | None = None, return_lse: bool = False):
+    """softmax(q k^T * scale) v over the cached tokens; q [B, Hq, T, D] fp16 or bf16 (any strides with unit dim
+    stride), Hq a multiple of the cache's heads (query head j reads kv head j // (Hq / H)).
+
+    lengths int32 [B] counts the cached tokens, the queries' own included; the n = counts[b] (None: T) query tokens
+    of a sequence are its last n, rows past n are padding.  causal: a query sees the keys up to its own position
+    (window > 0: only the last `window` of them); otherwise all lengths[b].  selected int32 [B, H, T, n]: each query
+    sees only these pages (kv_select_i8's result).  Rows that see no key are zero (lse -inf).
+
+    Writes `out` (default: a new [B, T, Hq, D] tensor, returned as its [B, Hq, T, D] view); with return_lse also
+    returns the natural log of each row's sum of exponentials, fp32 [B, Hq, T]."""
+    table, batch, width = _kv_table(cache, page_table)
+    heads, tokens = _kv_query(q, cache, batch)
+    dev, dim = cache.device, cache.head_dim
+    if out is None:
+        out = torch.empty((batch, tokens, heads, dim), device=dev, dtype=q.dtype).transpose(1, 2)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(3) != 1:
+        raise ValueError("out must have q's shape, dtype and device, and unit dim stride")
+    if lengths is None:
+        raise ValueError("lengths must be int32 [batch]")
+    n_sel = 0
+    if selected is not None:
+        if selected.ndim != 4 or not selected.shape[3]:
+            raise ValueError("selected must be int32 [batch, kv heads, tokens, pages]")
+        n_sel = selected.shape[3]
+        _kv_index(selected, "selected", (batch, cache.kv_heads, tokens, n_sel), dev)
+    lse = torch.empty((batch, heads, tokens), device=dev, dtype=F32) if return_lse else None
+    if tokens:
+        lib = _lib.load()
+        ws_bytes = lib.h3b_attention_kv_i8_workspace_size(batch, heads, cache.kv_heads, tokens, dim, width,
+                                                          cache.page_size, n_sel)
+        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+        _lib.check(lib.h3b_attention_kv_i8(
+            q.data_ptr(), _strides3(q), cache.struct, table, batch, width, _kv_index(lengths, "lengths", (batch,), dev),
+            _kv_index(counts, "counts", (batch,), dev), heads, tokens, float(scale), 1 if causal else 0, window,
+            _ptr(selected), n_sel, _KV_TYPES[q.dtype], out.data_ptr(), _strides3(out), _ptr(lse), ws.data_ptr(),
+            ws_bytes, _stream(dev)))
+        _count(1)
+    return (out, lse) if return_lse else out
+
+
+def kv_select_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.Tensor, pages: int, *,
+                 counts: torch.Tensor | None = None) -> torch.Tensor:
+    """The `pages` pages each query attends to: its own, and the earlier ones whose summed keys have the largest
+    product with the row-quantised query (the maximum over the group's heads; ties: the lower page).
+    q, lengths, counts as in attention_kv_i8; returns int32 [B, H, T, pages], ascending, -1 where none is left."""
+    table, batch, width = _kv_table(cache, page_table)
+    heads, tokens = _kv_query(q, cache, batch)
+    dev = cache.device
+    if pages < 1 or lengths is None:
+        raise ValueError("pages must be at least 1 and lengths int32 [batch]")
+    selected = torch.empty((batch, cache.kv_heads, tokens, pages), device=dev, dtype=_I32)
+    if tokens:
+        lib = _lib.load()
+        ws_bytes = lib.h3b_kv_select_i8_workspace_size(batch, cache.kv_heads, tokens, width)
+        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+        _lib.check(lib.h3b_kv_select_i8(
+            q.data_ptr(), _strides3(q), cache.struct, table, batch, width, _kv_index(lengths, "lengths", (batch,), dev),
+            _kv_index(counts, "counts", (batch,), dev), heads, tokens, pages, _KV_TYPES[q.dtype], selected.data_ptr(),
+            ws.data_ptr(), ws_bytes, _stream(dev)))
+        _count(2)
+    return selected
