@@ -1,585 +1,18 @@
-// Attention over the paged INT8 key/value cache.
-//
-// For a query row q at position p and the keys j it sees, with K codes kc, V
-// codes vc and their page's scales ks, vs:
-//   x_j = (q . kc_j) * (ks * scale * log2 e) + log2(vs),   m = max_j x_j,
-//   w_j = 2^(x_j - m) <= 1   (= the softmax weight times vs, up to a factor),
-//   out = sum_j w_j vc_j / sum_j (w_j / vs).
-// Folding vs into the exponent lets both products run on the codes themselves:
-// they are whole numbers, exact in fp16, so the only rounding of the inputs is
-// that of w to fp16, and scales that differ by any factor between pages stay
-// relative to the largest weighted one.
-#include "kv_common.cuh"
-
-namespace h3b {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-
-struct KvAttnParams {
-  KvView c;
-  const void* q;
-  void* out;
-  float* lse;
-  const int32_t* lengths;
-  const int32_t* counts;
-  const int32_t* selected;
-  int64_t qs[3], os[3];
-  int q_heads, group, tokens, n_selected, window;
-  bool causal, vec_q, vec_out;
-  float scale_log2;
-  // split plan (see attention_kv_split_kernel)
-  int row_tiles, slots, target, chunk;
-  float* part;     // [slot, kv head, row tile, row] x (dim + 2): weighted codes, m, l
-  int2* plan;      // per sequence: first slot, number of slots
-};
-
-// Tokens of sequence b, clamped to its table, and its number of query tokens.
-__device__ __forceinline__ int kv_length(const KvView& c, const int32_t* lengths, int b) {
-  const int len = max(lengths[b], 0);
-  if (len > c.width * c.page) {
-    record_error(kErrKvPage);
-    return c.width * c.page;
-  }
-  return len;
-}
-__device__ __forceinline__ int kv_count(const int32_t* counts, int tokens, int b) {
-  return counts ? max(0, min(counts[b], tokens)) : tokens;
-}
-
-// The keys [first, last) that query token t of n sees in a sequence of len
-// tokens, before any page selection; empty for padding rows.
-__device__ __forceinline__ void kv_range(const KvAttnParams& p, int len, int n, int t, int& first, int& last) {
-  const int pos = len - n + t;
-  first = last = 0;
-  if (t >= n || pos < 0) return;
-  last = p.causal ? pos + 1 : len;
-  if (p.window > 0) first = max(0, pos + 1 - p.window);
-}
-
-__device__ __forceinline__ float kv_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// D += A B, m16n8k16, fp16 operands, fp32 accumulators.
-__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Two codes as fp16: the bytes (sign bit flipped) become the low mantissa bits
-// of 1024.
-__device__ __forceinline__ uint32_t codes_to_h2(uint32_t biased, uint32_t selector) {
-  const uint32_t w = __byte_perm(biased, 0x64646464u, selector);
-  const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&w), __floats2half2_rn(1152.0f, 1152.0f));
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
-
-// A query row as fp16.  bf16 rows are scaled by a power of two so that their
-// largest value lies in [1, 2): every value that matters at fp32 precision of
-// the product is then exact in fp16; `back` undoes the scaling.
-__device__ __forceinline__ float row_scaling(__half, float, float& back) {
-  back = 1.0f;
-  return 1.0f;
-}
-__device__ __forceinline__ float row_scaling(__nv_bfloat16, float top, float& back) {
-  int e = static_cast<int>((__float_as_uint(top) >> 23) & 255u) - 127;
-  e = top == 0.0f ? 0 : max(-126, min(126, e));
-  back = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-  return __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-}
-
-// ---------------------------------------------------------------------------
-// Few query rows: keys split over blocks, joined by a second kernel
-// ---------------------------------------------------------------------------
-// A block takes 16 rows (query tokens x heads of one group) and a run of key
-// tiles; its warps take the tiles in turn, each with its own ring of shared
-// memory that bulk copies fill (a page's codes of one head are contiguous).
-// Codes go from shared memory straight into the m16n8k16 operand layout: a
-// dot product does not care in which order dims are taken, nor a weighted sum
-// in which order keys are, so each thread reads 16 consecutive bytes of a key
-// (four k-steps of K) or D/8 consecutive dims of four keys (a k-step of V).
-// With at most 8 rows the rows 8..15 of the second product carry what fp16
-// rounds off the weights, so that rounding costs nothing.
-//
-// The rows see nearly all keys of their sequence, so a call moves the cache's
-// bytes once and is bound by HBM when it is long and by latency (table, scale
-// and code loads in a row, then the join) when it is short.
-constexpr int kSplitWarps = 4;
-constexpr int kSplitStages = 3;
-constexpr int kSplitRows = 16;
-constexpr int kSplitPages = 768;      // pages a block's run of tiles may span (two blocks' shared memory fits an SM)
-constexpr int kSplitStageBytes = 8192;
-
-template <int D>
-struct KvSplit {
-  static constexpr int kKeys = kSplitStageBytes / 2 / D;    // keys per tile: 64 or 32
-  static constexpr int kRing = kSplitWarps * kSplitStages * kSplitStageBytes;
-  static constexpr int kMeta = kSplitPages * 16 + kSplitPages * 4;
-  static constexpr int kSmem = kRing + kMeta + kSplitWarps * kSplitStages * 8 + 128;
-};
-
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
-
-// Tiles a sequence's rows need, in tiles of `keys`.
-__device__ __forceinline__ int split_tiles(const KvAttnParams& p, int b, int keys, int& tile0) {
-  const int len = kv_length(p.c, p.lengths, b), n = kv_count(p.counts, p.tokens, b);
-  int first, last, unused;
-  const int t0 = max(0, n - len);             // the first row that has a position
-  kv_range(p, len, n, t0, first, unused);
-  kv_range(p, len, n, n - 1, unused, last);
-  tile0 = first / keys;
-  return last > first ? (last + keys - 1) / keys - tile0 : 0;
-}
-
-template <typename T, int D, bool kSparse, bool kSmall>
-__global__ void __launch_bounds__(32 * kSplitWarps, 2) attention_kv_split_kernel(const KvAttnParams p) {
-  using S = KvSplit<D>;
-  constexpr int KT = S::kKeys, kTiles = KT / 8, kSteps = D / 16, kThreads = 32 * kSplitWarps;
-  extern __shared__ __align__(128) uint8_t smem[];
-  float4* s_meta = reinterpret_cast<float4*>(smem + S::kRing);                 // per page: x scale, log2 vs, 1/vs
-  int* s_page = reinterpret_cast<int*>(s_meta + kSplitPages);                  // pool page, -1: none
-  uint64_t* s_bar = reinterpret_cast<uint64_t*>(s_page + kSplitPages);
-  int* s_red = reinterpret_cast<int*>(s_bar + kSplitWarps * kSplitStages);     // 4 ints
-
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
-  const int hk = blockIdx.y;
-
-  // ---- which sequence, rows and tiles ----
-  int b, t_sparse = 0, rt, slot, split, splits, tile0, tile1;
-  if (kSparse) {
-    b = blockIdx.z;
-    int x = blockIdx.x;
-    split = x % p.slots;
-    x /= p.slots;
-    rt = x % p.row_tiles;
-    t_sparse = x / p.row_tiles;
-    splits = p.slots;
-    slot = (b * p.tokens + t_sparse) * p.slots + split;
-    const int tiles = (p.n_selected * p.c.page + KT - 1) / KT;
-    tile0 = min(split * p.chunk, tiles);
-    tile1 = min(tile0 + p.chunk, tiles);
-  } else {
-    rt = blockIdx.x / p.slots;
-    slot = blockIdx.x % p.slots;
-    // equal chunks of tiles for the whole batch: every block scans the lengths
-    const int per = (p.c.batch + kThreads - 1) / kThreads;
-    const int b0 = tid * per, b1 = min(b0 + per, p.c.batch);
-    int sum = 0, base;
-    for (int i = b0; i < b1; ++i) sum += split_tiles(p, i, KT, base);
-    if (tid < 4) s_red[tid] = 0;
-    __syncthreads();
-    const int wsum = __reduce_add_sync(0xffffffffu, sum);
-    if (lane == 0) atomicAdd(&s_red[0], wsum);
-    __syncthreads();
-    const int64_t total = static_cast<int64_t>(s_red[0]) * p.c.heads * p.row_tiles;
-    const int chunk = static_cast<int>(min(max((total + p.target - 1) / p.target, static_cast<int64_t>(kSplitWarps)),
-                                           static_cast<int64_t>(p.chunk)));
-    int mine = 0;
-    for (int i = b0; i < b1; ++i) mine += max(1, (split_tiles(p, i, KT, base) + chunk - 1) / chunk);
-    int incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
-    }
-    __shared__ int s_warp[kSplitWarps];
-    if (lane == 31) s_warp[warp] = incl;
-    if (tid == 0) s_red[1] = -1;
-    __syncthreads();
-    int before = incl - mine;
-    for (int w = 0; w < warp; ++w) before += s_warp[w];
-    for (int i = b0; i < b1; ++i) {
-      int t0;
-      const int tiles = split_tiles(p, i, KT, t0);
-      const int n = max(1, (tiles + chunk - 1) / chunk);
-      if (slot >= before && slot < before + n) {
-        s_red[1] = i;
-        s_red[2] = before;
-        s_red[3] = n;
-      }
-      before += n;
-    }
-    __syncthreads();
-    b = s_red[1];
-    if (b < 0) return;
-    split = slot - s_red[2];
-    splits = s_red[3];
-    int t0;
-    const int tiles = split_tiles(p, b, KT, t0);
-    tile0 = t0 + min(split * chunk, tiles);
-    tile1 = t0 + min(split * chunk + chunk, tiles);
-    if (split == 0 && tid == 0 && hk == 0 && rt == 0 && p.plan) p.plan[b] = make_int2(s_red[2], splits);
-  }
-  const int len = kv_length(p.c, p.lengths, b), n_tok = kv_count(p.counts, p.tokens, b);
-
-  // ---- the pages of the run: numbers, then the first copies, then scales ----
-  const int page0 = (tile0 * KT) >> p.c.page_shift;
-  const int n_pages = tile1 > tile0 ? ((tile1 * KT - 1) >> p.c.page_shift) - page0 + 1 : 0;
-  const int32_t* sel =
-      kSparse ? p.selected + ((static_cast<int64_t>(b) * p.c.heads + hk) * p.tokens + t_sparse) * p.n_selected : nullptr;
-  for (int i = tid; i < n_pages; i += kThreads) {
-    int ord = page0 + i;
-    if (kSparse) ord = ord < p.n_selected ? sel[ord] : -1;
-    int page = -1;
-    if (ord >= 0 && static_cast<int64_t>(ord) * p.c.page < len) page = kv_page(p.c, b, ord);
-    s_page[i] = page;
-  }
-  if (tid < kSplitWarps * kSplitStages) mbar_init(&s_bar[tid], 1);
-  if (tid == 0) fence_barrier_init();
-  __syncthreads();
-
-  const uint32_t ring = smem_u32(smem) + warp * kSplitStages * kSplitStageBytes;
-  const uint32_t bars = smem_u32(s_bar + warp * kSplitStages);
-  const int seg_keys = min(p.c.page, KT);
-  const uint32_t seg_bytes = seg_keys * D;
-  auto issue = [&](int tile, int stage) {
-    // lane j copies the j-th segment (a page or the part of it in this tile)
-    const int key = tile * KT + lane * seg_keys;
-    int page = -1;
-    if (lane * seg_keys < KT) page = s_page[(key >> p.c.page_shift) - page0];
-    const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
-    const uint32_t bar = bars + stage * 8;
-    if (lane == 0)
-      asm volatile(
-          "{\n\t.reg .b64 st;\n\t"
-          "mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar),
-          "r"(2 * seg_bytes * __popc(there))
-          : "memory");
-    __syncwarp();
-    if (page >= 0) {
-      const int64_t off = ((static_cast<int64_t>(page) * p.c.heads + hk) * p.c.page + (key & (p.c.page - 1))) * D;
-      const uint32_t dst = ring + stage * kSplitStageBytes + lane * seg_bytes;
-      bulk_load(dst, p.c.code[0] + off, seg_bytes, bar);
-      bulk_load(dst + KT * D, p.c.code[1] + off, seg_bytes, bar);
-    }
-  };
-  for (int s = 0; s < kSplitStages; ++s) {
-    const int tile = tile0 + warp + s * kSplitWarps;
-    if (tile < tile1) issue(tile, s);
-  }
-  for (int i = tid; i < n_pages; i += kThreads) {
-    const int page = s_page[i];
-    float4 f = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);   // no page: weight 0
-    if (page >= 0) {
-      const int64_t ph = static_cast<int64_t>(page) * p.c.heads + hk;
-      float vs = p.c.scale[1][ph];
-      vs = vs < kKvMinScale ? kKvMinScale : vs;            // a page never written holds zeros; NaN stays
-      f = make_float4(p.c.scale[0][ph] * p.scale_log2, log2f(vs), __frcp_rn(vs), 0.0f);
-    }
-    if (kSparse && page >= 0) f.w = __int_as_float(sel[page0 + i] << p.c.page_shift);   // first position
-    s_meta[i] = f;
-  }
-
-  // ---- the query rows ----
-  const int g_rows = kSparse ? p.group : p.group * p.tokens;      // rows of this (sequence, kv head)
-  uint32_t qa[kSteps][4];
-  float back[2];
-  int first[2], last[2];
-  int first_max = 0, last_min = 0x7fffffff;
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int row = rt * kSplitRows + r + 8 * u;
-    const bool real = row < g_rows && !(kSmall && u == 1);
-    const int t = kSparse ? t_sparse : row / p.group, h = hk * p.group + (kSparse ? row : row % p.group);
-    first[u] = 0, last[u] = 0x7fffffff;      // padding rows never force masking
-    if (real) kv_range(p, len, n_tok, t, first[u], last[u]);
-    first_max = max(first_max, first[u]);
-    last_min = min(last_min, last[u]);
-    float x[D / 4];
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < D / 4; ++i) x[i] = 0.0f;
-    if (real) {
-      const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1] + t * p.qs[2];
-#pragma unroll
-      for (int v = 0; v < D / 64; ++v)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          load8(q + 64 * v + 16 * c + 8 * i, p.vec_q, *reinterpret_cast<float(*)[8]>(&x[16 * v + 8 * i]));
-    }
-#pragma unroll
-    for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const float f = row_scaling(T(), top, back[u]);
-    // k index 2c + e of step s is dim 64 (s / 4) + 16 c + 4 (s % 4) + e, and 2c + 8 + e the dim two further
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int i = 16 * (s >> 2) + 4 * (s & 3) + 2 * e;
-        qa[s][u + 2 * e] = h2_bits(__floats2half2_rn(x[i] * f, x[i + 1] * f));
-      }
-  }
-#pragma unroll
-  for (int o = 4; o < 32; o <<= 1) {
-    first_max = max(first_max, __shfl_xor_sync(0xffffffffu, first_max, o));
-    last_min = min(last_min, __shfl_xor_sync(0xffffffffu, last_min, o));
-  }
-  __syncthreads();   // scales are in shared memory
-
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-  float o[D / 8][4];
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-  constexpr int kU = kSmall ? 1 : 2;
-  // column j of an S tile is key (j >> 1) + 4 (j & 1) of its eight, so that the
-  // four keys a V load touches at once are neighbours
-  const int k_row = (r >> 1) + 4 * (r & 1);
-  bool ok = true;
-  int stage = 0, tile = tile0 + warp;
-  uint32_t phase = 0;
-  for (; tile < tile1; tile += kSplitWarps) {
-    ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(bars + stage * 8, phase, nullptr));
-    if (!ok) break;
-    const uint32_t ks = ring + stage * kSplitStageBytes, vs = ks + KT * D;
-    // S = Q K^T
-    float x[kTiles][4];
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      x[t][0] = x[t][1] = x[t][2] = x[t][3] = 0.0f;
-#pragma unroll
-      for (int v = 0; v < D / 64; ++v) {
-        uint4 w = ld_shared_v4(ks + (8 * t + k_row) * D + 64 * v + 16 * c);
-        const uint32_t ww[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-          mma_16816(x[t], qa[4 * v + s], codes_to_h2(ww[s], 0x4140), codes_to_h2(ww[s], 0x4342));
-      }
-    }
-    // scores in base 2 with log2 of the V scale; masked where a row does not see the key
-    float inv[kTiles / 2];
-    float top[2] = {-INFINITY, -INFINITY};
-    const int key0 = tile * KT;
-    const bool clear = !kSparse && key0 >= first_max && key0 + KT <= last_min;
-#pragma unroll
-    for (int t2 = 0; t2 < kTiles / 2; ++t2) {
-      const float4 f = s_meta[((key0 + 16 * t2) >> p.c.page_shift) - page0];
-      inv[t2] = f.z;
-#pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        const float sc = f.x * back[u];
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float& y = x[2 * t2 + tt][2 * u + e];
-            y = __fmaf_rn(y, sc, f.y);
-            if (!clear) {
-              const int in = 16 * t2 + 8 * tt + c + 4 * e;
-              const int key = kSparse ? __float_as_int(f.w) + ((key0 + in) & (p.c.page - 1)) : key0 + in;
-              if (key < first[u] || key >= last[u]) y = -INFINITY;
-            }
-            top[u] = fmaxf(top[u], y);
-          }
-      }
-    }
-    float ref[2];
-    bool moved = false;
-    float alpha[2];
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 1));
-      top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 2));
-      const float m_new = fmaxf(m[u], top[u]);
-      ref[u] = m_new == -INFINITY ? 0.0f : m_new;
-      moved |= m_new > m[u];
-      alpha[u] = kv_ex2(m[u] - ref[u]);
-      m[u] = m_new;
-    }
-    if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-      for (int u = 0; u < kU; ++u) l[u] *= alpha[u];
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        o[i][0] *= alpha[0];
-        o[i][1] *= alpha[0];
-        o[i][2] *= alpha[kSmall ? 0 : 1];
-        o[i][3] *= alpha[kSmall ? 0 : 1];
-      }
-    }
-    // weights, their sums, and O += W V
-#pragma unroll
-    for (int s = 0; s < kTiles / 2; ++s) {
-      uint32_t pa[4];
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-#pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          const float w0 = kv_ex2(x[2 * s + tt][2 * u] - ref[u]), w1 = kv_ex2(x[2 * s + tt][2 * u + 1] - ref[u]);
-          l[u] = __fmaf_rn(w0 + w1, inv[s], l[u]);
-          const __half2 hi = __floats2half2_rn(w0, w1);
-          pa[2 * tt + u] = h2_bits(hi);
-          if (kSmall) {
-            const float2 f = __half22float2(hi);
-            pa[2 * tt + 1] = h2_bits(__floats2half2_rn(w0 - f.x, w1 - f.y));
-          }
-        }
-      }
-      // keys 16 s + {c, c + 4, c + 8, c + 12}, dims D/8 r ..: words of four dims
-      uint32_t w[4][D / 32];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t at = vs + (16 * s + c + 4 * k) * D + (D / 8) * r;
-        if (D == 64) {
-          asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[k][0]), "=r"(w[k][1]) : "r"(at) : "memory");
-        } else {
-          const uint4 q4 = ld_shared_v4(at);
-          w[k][0] = q4.x, w[k][1] = q4.y, w[k][D / 32 - 2] = q4.z, w[k][D / 32 - 1] = q4.w;
-        }
-      }
-#pragma unroll
-      for (int d4 = 0; d4 < D / 32; ++d4) {
-        uint32_t lo[2], hi[2];   // key pairs interleaved: bytes (k0, k1) of dims 0, 1 and of dims 2, 3
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          lo[k] = __byte_perm(w[2 * k][d4], w[2 * k + 1][d4], 0x5140) ^ 0x80808080u;
-          hi[k] = __byte_perm(w[2 * k][d4], w[2 * k + 1][d4], 0x7362) ^ 0x80808080u;
-        }
-        mma_16816(o[4 * d4 + 0], pa, codes_to_h2(lo[0], 0x4140), codes_to_h2(lo[1], 0x4140));
-        mma_16816(o[4 * d4 + 1], pa, codes_to_h2(lo[0], 0x4342), codes_to_h2(lo[1], 0x4342));
-        mma_16816(o[4 * d4 + 2], pa, codes_to_h2(hi[0], 0x4140), codes_to_h2(hi[1], 0x4140));
-        mma_16816(o[4 * d4 + 3], pa, codes_to_h2(hi[0], 0x4342), codes_to_h2(hi[1], 0x4342));
-      }
-    }
-    __syncwarp();   // every lane has read the stage
-    const int next = tile + kSplitStages * kSplitWarps;
-    if (next < tile1) issue(next, stage);
-    if (++stage == kSplitStages) stage = 0, phase ^= 1;
-  }
-  if (!ok) {   // a wait gave up (the error word says so): let the copies issued after it land
-    for (int s = 1; s < kSplitStages; ++s) {
-      if (++stage == kSplitStages) stage = 0, phase ^= 1;
-      if (tile + s * kSplitWarps < tile1) mbar_wait_u32(bars + stage * 8, phase, nullptr);
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < kU; ++u) {
-    l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
-    l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
-  }
-
-  // ---- join the warps: thread (r, c) holds dims D/4 c .. of rows r and r + 8 ----
-  __syncthreads();   // all copies have landed and been read (every warp waited for each of its own)
-  constexpr int kOut = kSmall ? 8 : 16;
-  float* s_o = reinterpret_cast<float*>(smem);                       // [warp][row][D + 4]
-  float* s_ml = s_o + kSplitWarps * kOut * (D + 4);                  // [warp][row][2]
-  static_assert(kSplitWarps * kOut * (D + 6) * 4 <= S::kRing, "join buffer");
-#pragma unroll
-  for (int u = 0; u < kU; ++u) {
-    float* dst = s_o + (warp * kOut + r + 8 * u) * (D + 4) + (D / 4) * c;
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-      dst[i] = kSmall ? o[i][0] + o[i][2] : o[i][2 * u];
-      dst[D / 8 + i] = kSmall ? o[i][1] + o[i][3] : o[i][2 * u + 1];
-    }
-    if (c == 0) {
-      s_ml[(warp * kOut + r + 8 * u) * 2] = m[u];
-      s_ml[(warp * kOut + r + 8 * u) * 2 + 1] = l[u];
-    }
-  }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  __syncthreads();
-  const int rows = min(kOut, g_rows - rt * kSplitRows);
-  for (int i = tid; i < rows * (D / 4); i += kThreads) {
-    const int row = i / (D / 4), d = (i % (D / 4)) * 4;
-    float mm = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kSplitWarps; ++w) mm = fmaxf(mm, s_ml[(w * kOut + row) * 2]);
-    const float rf = mm == -INFINITY ? 0.0f : mm;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float ll = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kSplitWarps; ++w) {
-      const float f = kv_ex2(s_ml[(w * kOut + row) * 2] - rf);
-      const float4 v = *reinterpret_cast<const float4*>(s_o + (w * kOut + row) * (D + 4) + d);
-      acc.x = __fmaf_rn(f, v.x, acc.x);
-      acc.y = __fmaf_rn(f, v.y, acc.y);
-      acc.z = __fmaf_rn(f, v.z, acc.z);
-      acc.w = __fmaf_rn(f, v.w, acc.w);
-      ll = __fmaf_rn(f, s_ml[(w * kOut + row) * 2 + 1], ll);
-    }
-    const int full = rt * kSplitRows + row;
-    if (splits > 1) {
-      const int64_t at = ((static_cast<int64_t>(slot) * p.c.heads + hk) * p.row_tiles + rt) * kSplitRows + row;
-      *reinterpret_cast<float4*>(p.part + at * (D + 4) + d) = acc;
-      if (d == 0) *reinterpret_cast<float2*>(p.part + at * (D + 4) + D) = make_float2(mm, ll);
-    } else {
-      const int t = kSparse ? t_sparse : full / p.group, h = hk * p.group + (kSparse ? full : full % p.group);
-      const float f = ll == 0.0f ? 0.0f : __frcp_rn(ll);
-      T* out = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1] + t * p.os[2] + d;
-      from_f32(acc.x * f, out[0]);
-      from_f32(acc.y * f, out[1]);
-      from_f32(acc.z * f, out[2]);
-      from_f32(acc.w * f, out[3]);
-      if (p.lse && d == 0)
-        p.lse[(static_cast<int64_t>(b) * p.q_heads + h) * p.tokens + t] =
-            ll == 0.0f ? -INFINITY : (rf + log2f(ll)) * kLn2;
-    }
-  }
-}
-
-// Joins the slots of a row: one warp per row, D / 32 dims a lane.
-template <typename T, int D, bool kSparse>
-__global__ void __launch_bounds__(128) attention_kv_join_kernel(const KvAttnParams p) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int hk = blockIdx.y, b = blockIdx.z;
-  const int full = blockIdx.x * 4 + warp;          // row of the (sequence, kv head): token * group + head
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (full >= p.group * p.tokens) return;
-  const int t = full / p.group, g = full % p.group, h = hk * p.group + g;
-  int slot, n, rt, row;
-  if (kSparse) {
-    slot = (b * p.tokens + t) * p.slots;
-    n = p.slots;
-    rt = g / kSplitRows;
-    row = g % kSplitRows;
-  } else {
-    slot = p.plan[b].x;
-    n = p.plan[b].y;
-    rt = full / kSplitRows;
-    row = full % kSplitRows;
-  }
-  if (n <= 1) return;       // written by the block itself
-  const int64_t step = static_cast<int64_t>(p.c.heads) * p.row_tiles * kSplitRows * (D + 4);
-  const float* src = p.part + (((static_cast<int64_t>(slot) * p.c.heads + hk) * p.row_tiles + rt) * kSplitRows + row) * (D + 4);
-  float m = -INFINITY, l = 0.0f, o[D / 32] = {};
-  for (int s = 0; s < n; ++s, src += step) {
-    const float2 ml = *reinterpret_cast<const float2*>(src + D);
-    const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.0f : m_new;
-    const float a = kv_ex2(m - ref), f = kv_ex2(ml.x - ref);
-    m = m_new;
-    l = l * a + ml.y * f;
-#pragma unroll
-    for (int k = 0; k < D / 32; ++k) o[k] = o[k] * a + src[lane * (D / 32) + k] * f;
-  }
-  const float f = l == 0.0f ? 0.0f : __frcp_rn(l);
-  T* out = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1] + t * p.os[2] + lane * (D / 32);
-#pragma unroll
-  for (int k = 0; k < D / 32; ++k) from_f32(o[k] * f, out[k]);
-  if (p.lse && lane == 0)
-    p.lse[(static_cast<int64_t>(b) * p.q_heads + h) * p.tokens + t] =
-        l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) + log2f(l)) * kLn2;
-}
-
-}  // namespace h3b
+// Host side of attention over the paged INT8 cache: the choice between the
+// kernels of attention_kv_split.cu and attention_kv_tile.cu, workspaces, checks.
+#include "attention_kv.cuh"
 
 namespace {
 
-// The split plan of a call: rows in tiles of 16; `slots` runs of key tiles at
-// most (dense: over the whole batch, sparse: per query token).
+// Rows of a (sequence, kv head) above which the tensor-core tiles are taken.
+constexpr int64_t kTileRows = 64;
+
+// The plan of a call.  tile: attention_kv_tile_kernel, 256 rows a block, the
+// keys in `slots` parts.  Otherwise attention_kv_split_kernel: rows in tiles of
+// 16, `slots` runs of key tiles at most (dense: over the whole batch, sparse:
+// per query token).
 struct KvPlan {
+  bool tile;
   int64_t row_tiles, slots, chunk, target;
   size_t plan_bytes, part_bytes;
 };
@@ -592,6 +25,14 @@ KvPlan kv_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens,
   const int64_t keys = kSplitStageBytes / 2 / dim;
   const int64_t most = (kSplitPages - 1) * page / keys;    // tiles a run may have: it may start inside a page
   const int64_t rows = n_selected > 0 ? group : group * tokens;
+  k.tile = n_selected <= 0 && rows > kTileRows;
+  if (k.tile) {
+    k.row_tiles = (rows + 2 * kKtRows - 1) / (2 * kKtRows);
+    const int64_t blocks = batch * kv_heads * k.row_tiles, most_blocks = (width * page + kKtKeys - 1) / kKtKeys;
+    k.slots = std::max<int64_t>(1, std::min(h3b_host::num_sms() / blocks, most_blocks / 4));
+    k.part_bytes = k.slots > 1 ? (size_t)(k.slots * batch * kv_heads * rows) * (dim + 4) * 4 : 0;
+    return k;
+  }
   k.row_tiles = (rows + kSplitRows - 1) / kSplitRows;
   k.target = 4 * 2 * h3b_host::num_sms();                  // four blocks for each of the two an SM holds
   if (n_selected > 0) {
@@ -613,6 +54,23 @@ KvPlan kv_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens,
   return k;
 }
 
+template <typename T, int D, h3b::KvParts kParts>
+int launch_kv_join(const char* name, const h3b::KvAttnParams& p, int64_t batch, cudaStream_t st) {
+  using namespace h3b;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(((int64_t)p.group * p.tokens + 3) / 4), (unsigned)p.c.heads, (unsigned)batch);
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};   // the join's blocks may be resident before the parts are done; they wait for them
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, attention_kv_join_kernel<T, D, kParts>, p);
+  if (e != cudaSuccess) return h3b_host::set_error(H3B_ECUDA, "%s: join launch: %s", name, cudaGetErrorString(e));
+  return h3b_host::check_launch(name);
+}
+
 template <typename T, int D, bool kSparse>
 int launch_kv_split(const char* name, const h3b::KvAttnParams& p, int64_t batch, cudaStream_t st) {
   using namespace h3b;
@@ -626,23 +84,26 @@ int launch_kv_split(const char* name, const h3b::KvAttnParams& p, int64_t batch,
   kernel<<<dim3((unsigned)x, (unsigned)p.c.heads, kSparse ? (unsigned)batch : 1u), 32 * kSplitWarps, smem, st>>>(p);
   int rc = h3b_host::check_launch(name);
   if (rc || p.part == nullptr) return rc;
-  cudaLaunchConfig_t cfg{};
-  const int64_t all = (int64_t)p.group * p.tokens;
-  cfg.gridDim = dim3((unsigned)((all + 3) / 4), (unsigned)p.c.heads, (unsigned)batch);
-  cfg.blockDim = dim3(128);
-  cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, attention_kv_join_kernel<T, D, kSparse>, p);
-  if (e != cudaSuccess) return h3b_host::set_error(H3B_ECUDA, "%s: join launch: %s", name, cudaGetErrorString(e));
-  return h3b_host::check_launch(name);
+  return launch_kv_join<T, D, kSparse ? kPartsSparse : kPartsPlan>(name, p, batch, st);
 }
 
 template <typename T, int D>
-int launch_kv_attention(const char* name, const h3b::KvAttnParams& p, int64_t batch, cudaStream_t st) {
+int launch_kv_tile(const char* name, const h3b::KvAttnParams& p, int64_t batch, cudaStream_t st) {
+  using namespace h3b;
+  auto kernel = attention_kv_tile_kernel<T, D>;
+  constexpr int smem = KvTile<D>::kSmem;
+  static_assert(smem <= 232448, "shared memory budget");
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return h3b_host::set_error(H3B_ECUDA, "%s: smem attribute: %s", name, cudaGetErrorString(e));
+  kernel<<<dim3((unsigned)(p.row_tiles * p.slots), (unsigned)p.c.heads, (unsigned)batch), kKtThreads, smem, st>>>(p);
+  int rc = h3b_host::check_launch(name);
+  if (rc || p.part == nullptr) return rc;
+  return launch_kv_join<T, D, kPartsTile>(name, p, batch, st);
+}
+
+template <typename T, int D>
+int launch_kv_attention(const char* name, const h3b::KvAttnParams& p, bool tile, int64_t batch, cudaStream_t st) {
+  if (tile) return launch_kv_tile<T, D>(name, p, batch, st);
   return p.selected ? launch_kv_split<T, D, true>(name, p, batch, st) : launch_kv_split<T, D, false>(name, p, batch, st);
 }
 
@@ -690,10 +151,12 @@ extern "C" int h3b_attention_kv_i8(const void* q, const int64_t* q_strides, cons
   p.counts = counts;
   p.selected = selected;
   p.vec_q = h3b_host::aligned16(q);
+  p.vec_out = h3b_host::aligned16(out);
   for (int i = 0; i < 3; ++i) {
     p.qs[i] = q_strides[i];
     p.os[i] = out_strides[i];
     p.vec_q = p.vec_q && q_strides[i] % 8 == 0;
+    p.vec_out = p.vec_out && out_strides[i] % 8 == 0;
   }
   p.q_heads = (int)q_heads;
   p.group = (int)(q_heads / cache->kv_heads);
@@ -711,7 +174,7 @@ extern "C" int h3b_attention_kv_i8(const void* q, const int64_t* q_strides, cons
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool wide = cache->head_dim == 128;
   if (dtype == H3B_TYPE_F16)
-    return wide ? launch_kv_attention<__half, 128>(name, p, batch, st) : launch_kv_attention<__half, 64>(name, p, batch, st);
-  return wide ? launch_kv_attention<__nv_bfloat16, 128>(name, p, batch, st)
-              : launch_kv_attention<__nv_bfloat16, 64>(name, p, batch, st);
+    return wide ? launch_kv_attention<__half, 128>(name, p, k.tile, batch, st) : launch_kv_attention<__half, 64>(name, p, k.tile, batch, st);
+  return wide ? launch_kv_attention<__nv_bfloat16, 128>(name, p, k.tile, batch, st)
+              : launch_kv_attention<__nv_bfloat16, 64>(name, p, k.tile, batch, st);
 }

@@ -1,0 +1,499 @@
+// Attention over the paged INT8 cache for few query rows: keys split over
+// blocks, joined by a second kernel (the mathematics: attention_kv.cuh).
+#include "attention_kv.cuh"
+
+namespace h3b {
+
+// D += A B, m16n8k16, fp16 operands, fp32 accumulators.
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A block takes 16 rows (query tokens x heads of one group) and a run of key
+// tiles; its warps take the tiles in turn, each with its own ring of shared
+// memory that bulk copies fill (a page's codes of one head are contiguous).
+// Codes go from shared memory straight into the m16n8k16 operand layout: a
+// dot product does not care in which order dims are taken, nor a weighted sum
+// in which order keys are, so each thread reads 16 consecutive bytes of a key
+// (four k-steps of K) or D/8 consecutive dims of four keys (a k-step of V).
+// With at most 8 rows the rows 8..15 of the second product carry what fp16
+// rounds off the weights, so that rounding costs nothing.
+//
+// The rows see nearly all keys of their sequence, so a call moves the cache's
+// bytes once and is bound by HBM when it is long and by latency (table, scale
+// and code loads in a row, then the join) when it is short.
+constexpr int kSplitWarps = 4;
+constexpr int kSplitStages = 3;
+constexpr int kSplitRows = 16;
+constexpr int kSplitPages = 768;      // pages a block's run of tiles may span (two blocks' shared memory fits an SM)
+constexpr int kSplitStageBytes = 8192;
+
+template <int D>
+struct KvSplit {
+  static constexpr int kKeys = kSplitStageBytes / 2 / D;    // keys per tile: 64 or 32
+  static constexpr int kRing = kSplitWarps * kSplitStages * kSplitStageBytes;
+  static constexpr int kMeta = kSplitPages * 16 + kSplitPages * 4;
+  static constexpr int kSmem = kRing + kMeta + kSplitWarps * kSplitStages * 8 + 128;
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+// Tiles a sequence's rows need, in tiles of `keys`.
+__device__ __forceinline__ int split_tiles(const KvAttnParams& p, int b, int keys, int& tile0) {
+  const int len = kv_length(p.c, p.lengths, b), n = kv_count(p.counts, p.tokens, b);
+  int first, last, unused;
+  const int t0 = max(0, n - len);             // the first row that has a position
+  kv_range(p, len, n, t0, first, unused);
+  kv_range(p, len, n, n - 1, unused, last);
+  tile0 = first / keys;
+  return last > first ? (last + keys - 1) / keys - tile0 : 0;
+}
+
+template <typename T, int D, bool kSparse, bool kSmall>
+__global__ void __launch_bounds__(32 * kSplitWarps, 2) attention_kv_split_kernel(const KvAttnParams p) {
+  using S = KvSplit<D>;
+  constexpr int KT = S::kKeys, kTiles = KT / 8, kSteps = D / 16, kThreads = 32 * kSplitWarps;
+  extern __shared__ __align__(128) uint8_t smem[];
+  float4* s_meta = reinterpret_cast<float4*>(smem + S::kRing);                 // per page: x scale, log2 vs, 1/vs
+  int* s_page = reinterpret_cast<int*>(s_meta + kSplitPages);                  // pool page, -1: none
+  uint64_t* s_bar = reinterpret_cast<uint64_t*>(s_page + kSplitPages);
+  int* s_red = reinterpret_cast<int*>(s_bar + kSplitWarps * kSplitStages);     // 4 ints
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
+  const int hk = blockIdx.y;
+
+  // ---- which sequence, rows and tiles ----
+  int b, t_sparse = 0, rt, slot, split, splits, tile0, tile1;
+  if (kSparse) {
+    b = blockIdx.z;
+    int x = blockIdx.x;
+    split = x % p.slots;
+    x /= p.slots;
+    rt = x % p.row_tiles;
+    t_sparse = x / p.row_tiles;
+    splits = p.slots;
+    slot = (b * p.tokens + t_sparse) * p.slots + split;
+    const int tiles = (p.n_selected * p.c.page + KT - 1) / KT;
+    tile0 = min(split * p.chunk, tiles);
+    tile1 = min(tile0 + p.chunk, tiles);
+  } else {
+    rt = blockIdx.x / p.slots;
+    slot = blockIdx.x % p.slots;
+    // equal chunks of tiles for the whole batch: every block scans the lengths
+    const int per = (p.c.batch + kThreads - 1) / kThreads;
+    const int b0 = tid * per, b1 = min(b0 + per, p.c.batch);
+    int sum = 0, base;
+    for (int i = b0; i < b1; ++i) sum += split_tiles(p, i, KT, base);
+    if (tid < 4) s_red[tid] = 0;
+    __syncthreads();
+    const int wsum = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == 0) atomicAdd(&s_red[0], wsum);
+    __syncthreads();
+    const int64_t total = static_cast<int64_t>(s_red[0]) * p.c.heads * p.row_tiles;
+    const int chunk = static_cast<int>(min(max((total + p.target - 1) / p.target, static_cast<int64_t>(kSplitWarps)),
+                                           static_cast<int64_t>(p.chunk)));
+    int mine = 0;
+    for (int i = b0; i < b1; ++i) mine += max(1, (split_tiles(p, i, KT, base) + chunk - 1) / chunk);
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    __shared__ int s_warp[kSplitWarps];
+    if (lane == 31) s_warp[warp] = incl;
+    if (tid == 0) s_red[1] = -1;
+    __syncthreads();
+    int before = incl - mine;
+    for (int w = 0; w < warp; ++w) before += s_warp[w];
+    for (int i = b0; i < b1; ++i) {
+      int t0;
+      const int tiles = split_tiles(p, i, KT, t0);
+      const int n = max(1, (tiles + chunk - 1) / chunk);
+      if (slot >= before && slot < before + n) {
+        s_red[1] = i;
+        s_red[2] = before;
+        s_red[3] = n;
+      }
+      before += n;
+    }
+    __syncthreads();
+    b = s_red[1];
+    if (b < 0) return;
+    split = slot - s_red[2];
+    splits = s_red[3];
+    int t0;
+    const int tiles = split_tiles(p, b, KT, t0);
+    tile0 = t0 + min(split * chunk, tiles);
+    tile1 = t0 + min(split * chunk + chunk, tiles);
+    if (split == 0 && tid == 0 && hk == 0 && rt == 0 && p.plan) p.plan[b] = make_int2(s_red[2], splits);
+  }
+  const int len = kv_length(p.c, p.lengths, b), n_tok = kv_count(p.counts, p.tokens, b);
+
+  // ---- the pages of the run: numbers, then the first copies, then scales ----
+  const int page0 = (tile0 * KT) >> p.c.page_shift;
+  const int n_pages = tile1 > tile0 ? ((tile1 * KT - 1) >> p.c.page_shift) - page0 + 1 : 0;
+  const int32_t* sel =
+      kSparse ? p.selected + ((static_cast<int64_t>(b) * p.c.heads + hk) * p.tokens + t_sparse) * p.n_selected : nullptr;
+  for (int i = tid; i < n_pages; i += kThreads) {
+    int ord = page0 + i;
+    if (kSparse) ord = ord < p.n_selected ? sel[ord] : -1;
+    int page = -1;
+    if (ord >= 0 && static_cast<int64_t>(ord) * p.c.page < len) page = kv_page(p.c, b, ord);
+    s_page[i] = page;
+  }
+  if (tid < kSplitWarps * kSplitStages) mbar_init(&s_bar[tid], 1);
+  if (tid == 0) fence_barrier_init();
+  __syncthreads();
+
+  const uint32_t ring = smem_u32(smem) + warp * kSplitStages * kSplitStageBytes;
+  const uint32_t bars = smem_u32(s_bar + warp * kSplitStages);
+  const int seg_keys = min(p.c.page, KT);
+  const uint32_t seg_bytes = seg_keys * D;
+  auto issue = [&](int tile, int stage) {
+    // lane j copies the j-th segment (a page or the part of it in this tile)
+    const int key = tile * KT + lane * seg_keys;
+    int page = -1;
+    if (lane * seg_keys < KT) page = s_page[(key >> p.c.page_shift) - page0];
+    const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+    const uint32_t bar = bars + stage * 8;
+    if (lane == 0)
+      asm volatile(
+          "{\n\t.reg .b64 st;\n\t"
+          "mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar),
+          "r"(2 * seg_bytes * __popc(there))
+          : "memory");
+    __syncwarp();
+    if (page >= 0) {
+      const int64_t off = ((static_cast<int64_t>(page) * p.c.heads + hk) * p.c.page + (key & (p.c.page - 1))) * D;
+      const uint32_t dst = ring + stage * kSplitStageBytes + lane * seg_bytes;
+      bulk_load(dst, p.c.code[0] + off, seg_bytes, bar);
+      bulk_load(dst + KT * D, p.c.code[1] + off, seg_bytes, bar);
+    }
+  };
+  for (int s = 0; s < kSplitStages; ++s) {
+    const int tile = tile0 + warp + s * kSplitWarps;
+    if (tile < tile1) issue(tile, s);
+  }
+  for (int i = tid; i < n_pages; i += kThreads) {
+    const int page = s_page[i];
+    float4 f = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);   // no page: weight 0
+    if (page >= 0) {
+      const int64_t ph = static_cast<int64_t>(page) * p.c.heads + hk;
+      float vs = p.c.scale[1][ph];
+      vs = vs < kKvMinScale ? kKvMinScale : vs;            // a page never written holds zeros; NaN stays
+      f = make_float4(p.c.scale[0][ph] * p.scale_log2, log2f(vs), __frcp_rn(vs), 0.0f);
+    }
+    if (kSparse && page >= 0) f.w = __int_as_float(sel[page0 + i] << p.c.page_shift);   // first position
+    s_meta[i] = f;
+  }
+
+  // ---- the query rows ----
+  const int g_rows = kSparse ? p.group : p.group * p.tokens;      // rows of this (sequence, kv head)
+  uint32_t qa[kSteps][4];
+  float back[2];
+  int first[2], last[2];
+  int first_max = 0, last_min = 0x7fffffff;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int row = rt * kSplitRows + r + 8 * u;
+    const bool real = row < g_rows && !(kSmall && u == 1);
+    const int t = kSparse ? t_sparse : row / p.group, h = hk * p.group + (kSparse ? row : row % p.group);
+    first[u] = 0, last[u] = 0x7fffffff;      // padding rows never force masking
+    if (real) kv_range(p, len, n_tok, t, first[u], last[u]);
+    first_max = max(first_max, first[u]);
+    last_min = min(last_min, last[u]);
+    float x[D / 4];
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) x[i] = 0.0f;
+    if (real) {
+      const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1] + t * p.qs[2];
+#pragma unroll
+      for (int v = 0; v < D / 64; ++v)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          load8(q + 64 * v + 16 * c + 8 * i, p.vec_q, *reinterpret_cast<float(*)[8]>(&x[16 * v + 8 * i]));
+    }
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const float f = row_scaling(T(), top, back[u]);
+    // k index 2c + e of step s is dim 64 (s / 4) + 16 c + 4 (s % 4) + e, and 2c + 8 + e the dim two further
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = 16 * (s >> 2) + 4 * (s & 3) + 2 * e;
+        qa[s][u + 2 * e] = h2_bits(__floats2half2_rn(x[i] * f, x[i + 1] * f));
+      }
+  }
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) {
+    first_max = max(first_max, __shfl_xor_sync(0xffffffffu, first_max, o));
+    last_min = min(last_min, __shfl_xor_sync(0xffffffffu, last_min, o));
+  }
+  __syncthreads();   // scales are in shared memory
+
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  float o[D / 8][4];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+  constexpr int kU = kSmall ? 1 : 2;
+  // column j of an S tile is key (j >> 1) + 4 (j & 1) of its eight, so that the
+  // four keys a V load touches at once are neighbours
+  const int k_row = (r >> 1) + 4 * (r & 1);
+  bool ok = true;
+  int stage = 0, tile = tile0 + warp;
+  uint32_t phase = 0;
+  for (; tile < tile1; tile += kSplitWarps) {
+    ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(bars + stage * 8, phase, nullptr));
+    if (!ok) break;
+    const uint32_t ks = ring + stage * kSplitStageBytes, vs = ks + KT * D;
+    // S = Q K^T
+    float x[kTiles][4];
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+      x[t][0] = x[t][1] = x[t][2] = x[t][3] = 0.0f;
+#pragma unroll
+      for (int v = 0; v < D / 64; ++v) {
+        uint4 w = ld_shared_v4(ks + (8 * t + k_row) * D + 64 * v + 16 * c);
+        const uint32_t ww[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          mma_16816(x[t], qa[4 * v + s], codes_to_h2(ww[s], 0x4140), codes_to_h2(ww[s], 0x4342));
+      }
+    }
+    // scores in base 2 with log2 of the V scale; masked where a row does not see the key
+    float inv[kTiles / 2];
+    float top[2] = {-INFINITY, -INFINITY};
+    const int key0 = tile * KT;
+    const bool clear = !kSparse && key0 >= first_max && key0 + KT <= last_min;
+#pragma unroll
+    for (int t2 = 0; t2 < kTiles / 2; ++t2) {
+      const float4 f = s_meta[((key0 + 16 * t2) >> p.c.page_shift) - page0];
+      inv[t2] = f.z;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const float sc = f.x * back[u];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& y = x[2 * t2 + tt][2 * u + e];
+            y = __fmaf_rn(y, sc, f.y);
+            if (!clear) {
+              const int in = 16 * t2 + 8 * tt + c + 4 * e;
+              const int key = kSparse ? __float_as_int(f.w) + ((key0 + in) & (p.c.page - 1)) : key0 + in;
+              if (key < first[u] || key >= last[u]) y = -INFINITY;
+            }
+            top[u] = fmaxf(top[u], y);
+          }
+      }
+    }
+    float ref[2];
+    bool moved = false;
+    float alpha[2];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 1));
+      top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 2));
+      const float m_new = fmaxf(m[u], top[u]);
+      ref[u] = m_new == -INFINITY ? 0.0f : m_new;
+      moved |= m_new > m[u];
+      alpha[u] = ex2_approx(m[u] - ref[u]);
+      m[u] = m_new;
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int u = 0; u < kU; ++u) l[u] *= alpha[u];
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        o[i][0] *= alpha[0];
+        o[i][1] *= alpha[0];
+        o[i][2] *= alpha[kSmall ? 0 : 1];
+        o[i][3] *= alpha[kSmall ? 0 : 1];
+      }
+    }
+    // weights, their sums, and O += W V
+#pragma unroll
+    for (int s = 0; s < kTiles / 2; ++s) {
+      uint32_t pa[4];
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          const float w0 = ex2_approx(x[2 * s + tt][2 * u] - ref[u]), w1 = ex2_approx(x[2 * s + tt][2 * u + 1] - ref[u]);
+          l[u] = __fmaf_rn(w0 + w1, inv[s], l[u]);
+          const __half2 hi = __floats2half2_rn(w0, w1);
+          pa[2 * tt + u] = h2_bits(hi);
+          if (kSmall) {
+            const float2 f = __half22float2(hi);
+            pa[2 * tt + 1] = h2_bits(__floats2half2_rn(w0 - f.x, w1 - f.y));
+          }
+        }
+      }
+      // keys 16 s + {c, c + 4, c + 8, c + 12}, dims D/8 r ..: words of four dims
+      uint32_t w[4][D / 32];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t at = vs + (16 * s + c + 4 * k) * D + (D / 8) * r;
+        if (D == 64) {
+          asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[k][0]), "=r"(w[k][1]) : "r"(at) : "memory");
+        } else {
+          const uint4 q4 = ld_shared_v4(at);
+          w[k][0] = q4.x, w[k][1] = q4.y, w[k][D / 32 - 2] = q4.z, w[k][D / 32 - 1] = q4.w;
+        }
+      }
+#pragma unroll
+      for (int d4 = 0; d4 < D / 32; ++d4) {
+        uint32_t lo[2], hi[2];   // key pairs interleaved: bytes (k0, k1) of dims 0, 1 and of dims 2, 3
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          lo[k] = __byte_perm(w[2 * k][d4], w[2 * k + 1][d4], 0x5140) ^ 0x80808080u;
+          hi[k] = __byte_perm(w[2 * k][d4], w[2 * k + 1][d4], 0x7362) ^ 0x80808080u;
+        }
+        mma_16816(o[4 * d4 + 0], pa, codes_to_h2(lo[0], 0x4140), codes_to_h2(lo[1], 0x4140));
+        mma_16816(o[4 * d4 + 1], pa, codes_to_h2(lo[0], 0x4342), codes_to_h2(lo[1], 0x4342));
+        mma_16816(o[4 * d4 + 2], pa, codes_to_h2(hi[0], 0x4140), codes_to_h2(hi[1], 0x4140));
+        mma_16816(o[4 * d4 + 3], pa, codes_to_h2(hi[0], 0x4342), codes_to_h2(hi[1], 0x4342));
+      }
+    }
+    __syncwarp();   // every lane has read the stage
+    const int next = tile + kSplitStages * kSplitWarps;
+    if (next < tile1) issue(next, stage);
+    if (++stage == kSplitStages) stage = 0, phase ^= 1;
+  }
+  if (!ok) {   // a wait gave up (the error word says so): let the copies issued after it land
+    for (int s = 1; s < kSplitStages; ++s) {
+      if (++stage == kSplitStages) stage = 0, phase ^= 1;
+      if (tile + s * kSplitWarps < tile1) mbar_wait_u32(bars + stage * 8, phase, nullptr);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+    l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+  }
+
+  // ---- join the warps: thread (r, c) holds dims D/4 c .. of rows r and r + 8 ----
+  __syncthreads();   // all copies have landed and been read (every warp waited for each of its own)
+  constexpr int kOut = kSmall ? 8 : 16;
+  float* s_o = reinterpret_cast<float*>(smem);                       // [warp][row][D + 4]
+  float* s_ml = s_o + kSplitWarps * kOut * (D + 4);                  // [warp][row][2]
+  static_assert(kSplitWarps * kOut * (D + 6) * 4 <= S::kRing, "join buffer");
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    float* dst = s_o + (warp * kOut + r + 8 * u) * (D + 4) + (D / 4) * c;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      dst[i] = kSmall ? o[i][0] + o[i][2] : o[i][2 * u];
+      dst[D / 8 + i] = kSmall ? o[i][1] + o[i][3] : o[i][2 * u + 1];
+    }
+    if (c == 0) {
+      s_ml[(warp * kOut + r + 8 * u) * 2] = m[u];
+      s_ml[(warp * kOut + r + 8 * u) * 2 + 1] = l[u];
+    }
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __syncthreads();
+  const int rows = min(kOut, g_rows - rt * kSplitRows);
+  for (int i = tid; i < rows * (D / 4); i += kThreads) {
+    const int row = i / (D / 4), d = (i % (D / 4)) * 4;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kSplitWarps; ++w) mm = fmaxf(mm, s_ml[(w * kOut + row) * 2]);
+    const float rf = mm == -INFINITY ? 0.0f : mm;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float ll = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kSplitWarps; ++w) {
+      const float f = ex2_approx(s_ml[(w * kOut + row) * 2] - rf);
+      const float4 v = *reinterpret_cast<const float4*>(s_o + (w * kOut + row) * (D + 4) + d);
+      acc.x = __fmaf_rn(f, v.x, acc.x);
+      acc.y = __fmaf_rn(f, v.y, acc.y);
+      acc.z = __fmaf_rn(f, v.z, acc.z);
+      acc.w = __fmaf_rn(f, v.w, acc.w);
+      ll = __fmaf_rn(f, s_ml[(w * kOut + row) * 2 + 1], ll);
+    }
+    const int full = rt * kSplitRows + row;
+    if (splits > 1) {
+      const int64_t at = ((static_cast<int64_t>(slot) * p.c.heads + hk) * p.row_tiles + rt) * kSplitRows + row;
+      *reinterpret_cast<float4*>(p.part + at * (D + 4) + d) = acc;
+      if (d == 0) *reinterpret_cast<float2*>(p.part + at * (D + 4) + D) = make_float2(mm, ll);
+    } else {
+      const int t = kSparse ? t_sparse : full / p.group, h = hk * p.group + (kSparse ? full : full % p.group);
+      const float f = ll == 0.0f ? 0.0f : __frcp_rn(ll);
+      T* out = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1] + t * p.os[2] + d;
+      from_f32(acc.x * f, out[0]);
+      from_f32(acc.y * f, out[1]);
+      from_f32(acc.z * f, out[2]);
+      from_f32(acc.w * f, out[3]);
+      if (p.lse && d == 0)
+        p.lse[(static_cast<int64_t>(b) * p.q_heads + h) * p.tokens + t] =
+            ll == 0.0f ? -INFINITY : (rf + log2f(ll)) * kLn2;
+    }
+  }
+}
+
+// Joins the slots of a row: one warp per row, D / 32 dims a lane.
+enum KvParts { kPartsPlan, kPartsSparse, kPartsTile };   // how the parts of a row are laid out
+
+template <typename T, int D, KvParts kParts>
+__global__ void __launch_bounds__(128) attention_kv_join_kernel(const KvAttnParams p) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hk = blockIdx.y, b = blockIdx.z;
+  const int full = blockIdx.x * 4 + warp;          // row of the (sequence, kv head): token * group + head
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (full >= p.group * p.tokens) return;
+  const int t = full / p.group, g = full % p.group, h = hk * p.group + g;
+  int n;
+  int64_t at, step;      // in rows of the parts
+  if (kParts == kPartsTile) {
+    n = p.slots;
+    at = (static_cast<int64_t>(b) * p.c.heads + hk) * p.group * p.tokens + full;
+    step = static_cast<int64_t>(p.c.batch) * p.c.heads * p.group * p.tokens;
+  } else {
+    int slot, in = full;
+    if (kParts == kPartsSparse) {
+      slot = (b * p.tokens + t) * p.slots;
+      n = p.slots;
+      in = g;
+    } else {
+      slot = p.plan[b].x;
+      n = p.plan[b].y;
+    }
+    step = static_cast<int64_t>(p.c.heads) * p.row_tiles * kSplitRows;
+    at = slot * step + static_cast<int64_t>(hk) * p.row_tiles * kSplitRows + in;
+  }
+  if (n <= 1) return;       // written by the block itself
+  const float* src = p.part + at * (D + 4);
+  step *= D + 4;
+  float m = -INFINITY, l = 0.0f, o[D / 32] = {};
+  for (int s = 0; s < n; ++s, src += step) {
+    const float2 ml = *reinterpret_cast<const float2*>(src + D);
+    const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.0f : m_new;
+    const float a = ex2_approx(m - ref), f = ex2_approx(ml.x - ref);
+    m = m_new;
+    l = l * a + ml.y * f;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) o[k] = o[k] * a + src[lane * (D / 32) + k] * f;
+  }
+  const float f = l == 0.0f ? 0.0f : __frcp_rn(l);
+  T* out = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1] + t * p.os[2] + lane * (D / 32);
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) from_f32(o[k] * f, out[k]);
+  if (p.lse && lane == 0)
+    p.lse[(static_cast<int64_t>(b) * p.q_heads + h) * p.tokens + t] =
+        l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) + log2f(l)) * kLn2;
+}
+
+}  // namespace h3b

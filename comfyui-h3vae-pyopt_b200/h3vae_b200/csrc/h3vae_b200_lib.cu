@@ -8,5 +8,7 @@
 #include "conv_in.cu"
 #include "conv_rgb.cu"
 #include "kv_cache.cu"
+#include "attention_kv_split.cu"
+#include "attention_kv_tile.cu"
 #include "attention_kv.cu"
 #include "kv_select.cu"
