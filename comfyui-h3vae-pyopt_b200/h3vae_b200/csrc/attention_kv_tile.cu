@@ -16,8 +16,10 @@
 //                the next block; x = S * (ks * scale * log2 e) + log2 vs against
 //                the running maximum gives weights in fp16 for the second product
 //                and, times 1 / vs in fp32, the denominator.
-// The reference maximum moves only when a block's exceeds it by more than 8
-// (weights stay <= 256); O is rescaled in TMEM then.  The two row tiles take
+// The reference maximum is the first block's that a row sees; a later block is
+// taken against it as it is, and only when 16 of its weights sum to more than
+// 2^14 (fp16 holds 65504, and keeps its 11 bits up to there) is its own maximum
+// looked for, the block redone and O rescaled in TMEM.  The two row tiles take
 // turns on the SFU, so that one tile's exponentials overlap the other's products.
 // Blocks that no row of the CTA sees are not visited, and only blocks on an edge
 // of a row's range test each key.
@@ -30,7 +32,9 @@ constexpr int kKtKeys = 128;                 // keys per block
 constexpr int kKtConvWarps = 3;
 constexpr int kKtThreads = 32 * (kKtConvWarps + 1 + 8);   // three warps a scheduler: 168 registers a thread
 constexpr int kKtUnit = 64;                  // keys a converter warp takes at a time
+constexpr int kKtChunk = 64;                 // products of a row in registers at a time
 constexpr int kKtMeta = 8;                   // blocks whose scales are kept
+constexpr float kKtMostWeight = 16384.0f;    // sum of 16 weights above which their maximum moves
 
 template <int D>
 struct KvTile {
@@ -40,37 +44,39 @@ struct KvTile {
   static constexpr uint32_t kSmem = 2 * kTile + kSlots * kTile + 2 * kP + kKtMeta * 8 * 16 + 256 + 1024;
 };
 
-// A row's 128 products out of TMEM.  One statement with its wait, so that no use
-// of a register moves above it.
-__device__ __forceinline__ void tmem_ld128_wait(uint32_t taddr, uint32_t (&r)[128]) {
+// Some of a row's products out of TMEM.  One statement with its wait, so that no
+// use of a register moves above it.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t taddr, float (&r)[32]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31"
+      "}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+        "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+        "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+        "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait(uint32_t taddr, float (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
       "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
       "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
       "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
-      "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
-      "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
-      "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
-      "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127"
-      "}, [%128];\n\t"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63"
+      "}, [%64];\n\t"
       "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
-        "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
-        "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
-        "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
-        "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
-        "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
-        "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
-        "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
-        "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+        "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+        "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+        "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31]),
+        "=f"(r[32]), "=f"(r[33]), "=f"(r[34]), "=f"(r[35]), "=f"(r[36]), "=f"(r[37]), "=f"(r[38]), "=f"(r[39]),
+        "=f"(r[40]), "=f"(r[41]), "=f"(r[42]), "=f"(r[43]), "=f"(r[44]), "=f"(r[45]), "=f"(r[46]), "=f"(r[47]),
+        "=f"(r[48]), "=f"(r[49]), "=f"(r[50]), "=f"(r[51]), "=f"(r[52]), "=f"(r[53]), "=f"(r[54]), "=f"(r[55]),
+        "=f"(r[56]), "=f"(r[57]), "=f"(r[58]), "=f"(r[59]), "=f"(r[60]), "=f"(r[61]), "=f"(r[62]), "=f"(r[63])
       : "r"(taddr)
       : "memory");
 }
@@ -122,54 +128,63 @@ __device__ __forceinline__ float score_scale(float x_scale, float back) { return
 
 // The largest score of a row's 128 products, in base 2 with log2 vs; scales are
 // positive, so the largest product of 16 keys is found first.
-__device__ __forceinline__ float row_max(const uint32_t (&x)[128], uint32_t meta, float back) {
+__device__ __noinline__ float row_max(uint32_t taddr, uint32_t meta, float back) {
   float top = -INFINITY;
+#pragma unroll 1
+  for (int u = 0; u < 8; u += 2) {
+    float x[32];
+    tmem_ld_wait(taddr + 16 * u, x);
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    const uint32_t* v = x + 16 * u;
-    auto at = [v](int k) { return __uint_as_float(v[k]); };
-    float a = fmax3(at(0), at(1), at(2)), c = fmax3(at(3), at(4), at(5));
-    a = fmax3(a, at(6), at(7));
-    c = fmax3(c, at(8), at(9));
-    a = fmax3(a, at(10), at(11));
-    c = fmax3(c, at(12), at(13));
-    a = fmax3(a, at(14), at(15));
-    const float4 f = meta_load(meta + 16 * u);
-    top = fmaxf(top, __fmaf_rn(fmaxf(a, c), score_scale(f.x, back), f.y));
+    for (int v = 0; v < 2; ++v) {
+      float a = x[16 * v];
+#pragma unroll
+      for (int k = 1; k < 16; ++k) a = fmaxf(a, x[16 * v + k]);
+      const float4 f = meta_load(meta + 16 * (u + v));
+      top = fmaxf(top, __fmaf_rn(a, score_scale(f.x, back), f.y));
+    }
   }
   return top;
 }
 
-// Weights of the products, rounded to fp16 into the row of P; returns the sum of
-// weight / vs.
+// Weights of a row's products, rounded to fp16 into its row of P; returns the sum
+// of weight / vs, and in `most` a bound of the largest weight.  kKtChunk products
+// are in registers at a time: with all 128 the loop has no registers left to keep
+// the exponentials going.
 template <int D>
-__device__ __forceinline__ float weights(const uint32_t (&x)[128], uint32_t meta, float back, float ref, uint32_t prow,
-                                         int row) {
+__device__ __forceinline__ float weights(uint32_t taddr, uint32_t meta, float back, float ref, uint32_t prow, int row,
+                                         float& most) {
   float sum = 0.0f;
+  most = 0.0f;
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    const float4 f = meta_load(meta + 16 * u);
-    const float sc = score_scale(f.x, back), sh = f.y - ref;
-    uint64_t acc = 0;
+  for (int c = 0; c < kKtKeys / kKtChunk; ++c) {
+    float x[kKtChunk];
+    tmem_ld_wait(taddr + kKtChunk * c, x);
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
-      uint32_t w[4];
+    for (int u = 0; u < kKtChunk / 16; ++u) {
+      const float4 f = meta_load(meta + kKtChunk * c + 16 * u);
+      const float sc = score_scale(f.x, back), sh = f.y - ref;
+      uint64_t acc = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int k = 16 * u + 8 * v + 2 * e;
-        float x0, x1;
-        f2_unpack(f2_fma(f2_pack(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), f2_pack(sc, sc), f2_pack(sh, sh)),
-                  x0, x1);
-        const float w0 = ex2_approx(x0), w1 = ex2_approx(x1);
-        acc = f2_add(acc, f2_pack(w0, w1));
-        w[e] = h2_bits(__floats2half2_rn(w0, w1));
+      for (int v = 0; v < 2; ++v) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int k = 16 * u + 8 * v + 2 * e;
+          float x0, x1;
+          f2_unpack(f2_fma(f2_pack(x[k], x[k + 1]), f2_pack(sc, sc), f2_pack(sh, sh)), x0, x1);
+          const float w0 = ex2_approx(x0), w1 = ex2_approx(x1);
+          acc = f2_add(acc, f2_pack(w0, w1));
+          w[e] = h2_bits(__floats2half2_rn(w0, w1));
+        }
+        const int q = (kKtChunk / 8) * c + 2 * u + v;
+        st_shared_v4(prow + (q >> 3) * (KvTile<D>::kP / 2) + (((q & 7) ^ (row & 7)) << 4),
+                     make_uint4(w[0], w[1], w[2], w[3]));
       }
-      const int q = 2 * u + v;
-      st_shared_v4(prow + (q >> 3) * (KvTile<D>::kP / 2) + (((q & 7) ^ (row & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+      float a0, a1;
+      f2_unpack(acc, a0, a1);
+      most = fmaxf(most, a0 + a1);
+      sum = __fmaf_rn(a0 + a1, f.z, sum);
     }
-    float a0, a1;
-    f2_unpack(acc, a0, a1);
-    sum = __fmaf_rn(a0 + a1, f.z, sum);
   }
   return sum;
 }
@@ -390,9 +405,10 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
       };
       for (int t = 0; t < tiles && ok && n_blocks > 0; ++t) ok = issue_s(0, t);
       for (int j = 0; j < n_blocks && ok; ++j) {
-        for (int t = 0; t < tiles && ok && j + 1 < n_blocks; ++t) ok = issue_s(j + 1, t);
         const int seq = seq_v(j), s = seq % NS;
         for (int t = 0; t < tiles && ok; ++t) {
+          // the softmax of block j has left S(t): the next products first, they are waited for sooner
+          if (j + 1 < n_blocks && !issue_s(j + 1, t)) { ok = false; break; }
           if (t == 0 && !mbar_poll(&slot_full[s], (seq / NS) & 1, abort_flag)) { ok = false; break; }
           if (!mbar_poll(&p_full[t], j & 1, abort_flag)) { ok = false; break; }
           tc_fence_after();
@@ -455,8 +471,6 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
       const uint32_t prow = smem_u32(sp + tile * L::kP + row * 128);
       const uint32_t bar_s_full = smem_u32(&s_full[tile]), bar_s_empty = smem_u32(&s_empty[tile]);
       const uint32_t bar_p_full = smem_u32(&p_full[tile]), bar_o_full = smem_u32(&o_full[tile]);
-      const bool turns = tiles == 2;
-      if (turns && tile == 1 && n_blocks > 0) asm volatile("bar.arrive 1, 256;" ::: "memory");
       for (int j = 0; j < n_blocks; ++j) {
         ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(smem_u32(&meta_full[j % kKtMeta]), (j / kKtMeta) & 1, abort_flag));
         ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(bar_s_full, j & 1, abort_flag));
@@ -466,25 +480,29 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
         tc_fence_after();
         const int key0 = (blk0 + j) * kKtKeys;
         if (key0 < first_max || key0 + kKtKeys > last_min) mask_products(t_s, first - key0, last - key0);
-        uint32_t x[128];
-        tmem_ld128_wait(t_s, x);
+        if (j > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(bar_o_full, (j - 1) & 1, abort_flag));
+        // Against the maximum so far; only a row without one, or whose weights outgrow fp16's range by
+        // their sums, looks for this block's.
+        bool look = __any_sync(0xffffffffu, m == -INFINITY), moved = false;
+        float alpha = 1.0f, sum;
+        while (true) {
+          if (look) {
+            const float m_new = fmaxf(m, row_max(t_s, meta, back));
+            moved = m_new > m;
+            alpha = moved ? ex2_approx(m - m_new) : 1.0f;
+            m = m_new;
+          }
+          float most;
+          sum = weights<D>(t_s, meta, back, m == -INFINITY ? 0.0f : m, prow, row, most);
+          if (look || !__any_sync(0xffffffffu, most > kKtMostWeight)) break;
+          look = true;
+        }
         tc_fence_before();
         mbar_arrive_u32(bar_s_empty);
-        const float top = row_max(x, meta, back);
-        const bool move = top > m + 8.0f;
-        const float m_new = move ? top : m;
-        const float alpha = move ? ex2_approx(m - m_new) : 1.0f;
-        const float ref = m_new == -INFINITY ? 0.0f : m_new;
-        m = m_new;
-        if (j > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(bar_o_full, (j - 1) & 1, abort_flag));
-        if (turns) asm volatile("bar.sync %0, 256;" ::"r"(tile == 0 ? 1 : 2) : "memory");
-        const float sum = weights<D>(x, meta, back, ref, prow, row);
-        if (turns && (tile == 0 || j + 1 < n_blocks))
-          asm volatile("bar.arrive %0, 256;" ::"r"(tile == 0 ? 2 : 1) : "memory");
         l = __fmaf_rn(l, alpha, sum);
         if (ok && j > 0) {
           tc_fence_after();
-          if (__any_sync(0xffffffffu, move)) rescale_row(t_o, D, alpha);
+          if (__any_sync(0xffffffffu, moved)) rescale_row(t_o, D, alpha);
         }
         if (ok) {
           tc_fence_before();
