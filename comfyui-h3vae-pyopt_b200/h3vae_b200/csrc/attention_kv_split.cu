@@ -6,7 +6,7 @@ namespace h3b {
 
 // D += A B, m16n8k16, fp16 operands, fp32 accumulators.
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -26,9 +26,10 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
 // bytes once and is bound by HBM when it is long and by latency (table, scale
 // and code loads in a row, then the join) when it is short.
 constexpr int kSplitWarps = 4;
-constexpr int kSplitStages = 3;
+constexpr int kSplitStages = 2;
+constexpr int kSplitBlocks = 3;       // blocks an SM holds (two with three stages: 154 against 139 us on 16 x 32768 keys)
 constexpr int kSplitRows = 16;
-constexpr int kSplitPages = 768;      // pages a block's run of tiles may span (two blocks' shared memory fits an SM)
+constexpr int kSplitPages = 256;      // pages a block's run of tiles may span
 constexpr int kSplitStageBytes = 8192;
 
 template <int D>
@@ -57,7 +58,7 @@ __device__ __forceinline__ int split_tiles(const KvAttnParams& p, int b, int key
 }
 
 template <typename T, int D, bool kSparse, bool kSmall>
-__global__ void __launch_bounds__(32 * kSplitWarps, 2) attention_kv_split_kernel(const KvAttnParams p) {
+__global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_split_kernel(const KvAttnParams p) {
   using S = KvSplit<D>;
   constexpr int KT = S::kKeys, kTiles = KT / 8, kSteps = D / 16, kThreads = 32 * kSplitWarps;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -86,54 +87,66 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attention_kv_split_kernel
   } else {
     rt = blockIdx.x / p.slots;
     slot = blockIdx.x % p.slots;
-    // equal chunks of tiles for the whole batch: every block scans the lengths
-    const int per = (p.c.batch + kThreads - 1) / kThreads;
-    const int b0 = tid * per, b1 = min(b0 + per, p.c.batch);
-    int sum = 0, base;
-    for (int i = b0; i < b1; ++i) sum += split_tiles(p, i, KT, base);
-    if (tid < 4) s_red[tid] = 0;
-    __syncthreads();
-    const int wsum = __reduce_add_sync(0xffffffffu, sum);
-    if (lane == 0) atomicAdd(&s_red[0], wsum);
-    __syncthreads();
-    const int64_t total = static_cast<int64_t>(s_red[0]) * p.c.heads * p.row_tiles;
-    const int chunk = static_cast<int>(min(max((total + p.target - 1) / p.target, static_cast<int64_t>(kSplitWarps)),
-                                           static_cast<int64_t>(p.chunk)));
-    int mine = 0;
-    for (int i = b0; i < b1; ++i) mine += max(1, (split_tiles(p, i, KT, base) + chunk - 1) / chunk);
-    int incl = mine;
+    int t0, chunk, first_slot;
+    auto chunk_of = [&](int sum) {   // equal chunks of tiles for the whole batch
+      const int64_t total = static_cast<int64_t>(sum) * p.c.heads * p.row_tiles;
+      return static_cast<int>(min(max((total + p.target - 1) / p.target, static_cast<int64_t>(kSplitWarps)),
+                                  static_cast<int64_t>(p.chunk)));
+    };
+    if (p.c.batch == 1 || p.plan == nullptr) {       // one sequence, or none is split
+      b = p.plan == nullptr ? slot : 0;
+      const int tiles = split_tiles(p, b, KT, t0);
+      chunk = p.plan == nullptr ? max(tiles, 1) : chunk_of(tiles);
+      splits = max(1, (tiles + chunk - 1) / chunk);
+      first_slot = b;
+      if (slot >= first_slot + splits) return;
+    } else {                                         // every block scans the lengths
+      __shared__ int s_warp[kSplitWarps];
+      const int per = (p.c.batch + kThreads - 1) / kThreads;
+      const int b0 = tid * per, b1 = min(b0 + per, p.c.batch);
+      int sum = 0, base;
+      for (int i = b0; i < b1; ++i) sum += split_tiles(p, i, KT, base);
+      sum = __reduce_add_sync(0xffffffffu, sum);
+      if (lane == 0) s_warp[warp] = sum;
+      if (tid == 0) s_red[0] = -1;
+      __syncthreads();
+      sum = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
-    }
-    __shared__ int s_warp[kSplitWarps];
-    if (lane == 31) s_warp[warp] = incl;
-    if (tid == 0) s_red[1] = -1;
-    __syncthreads();
-    int before = incl - mine;
-    for (int w = 0; w < warp; ++w) before += s_warp[w];
-    for (int i = b0; i < b1; ++i) {
-      int t0;
-      const int tiles = split_tiles(p, i, KT, t0);
-      const int n = max(1, (tiles + chunk - 1) / chunk);
-      if (slot >= before && slot < before + n) {
-        s_red[1] = i;
-        s_red[2] = before;
-        s_red[3] = n;
+      for (int w = 0; w < kSplitWarps; ++w) sum += s_warp[w];
+      chunk = chunk_of(sum);
+      int mine = 0;
+      for (int i = b0; i < b1; ++i) mine += max(1, (split_tiles(p, i, KT, base) + chunk - 1) / chunk);
+      int incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
       }
-      before += n;
+      __syncthreads();
+      if (lane == 31) s_warp[warp] = incl;
+      __syncthreads();
+      int before = incl - mine;
+      for (int w = 0; w < warp; ++w) before += s_warp[w];
+      for (int i = b0; i < b1; ++i) {
+        const int n = max(1, (split_tiles(p, i, KT, t0) + chunk - 1) / chunk);
+        if (slot >= before && slot < before + n) {
+          s_red[0] = i;
+          s_red[1] = before;
+          s_red[2] = n;
+        }
+        before += n;
+      }
+      __syncthreads();
+      b = s_red[0];
+      if (b < 0) return;
+      first_slot = s_red[1];
+      splits = s_red[2];
     }
-    __syncthreads();
-    b = s_red[1];
-    if (b < 0) return;
-    split = slot - s_red[2];
-    splits = s_red[3];
-    int t0;
+    split = slot - first_slot;
     const int tiles = split_tiles(p, b, KT, t0);
     tile0 = t0 + min(split * chunk, tiles);
     tile1 = t0 + min(split * chunk + chunk, tiles);
-    if (split == 0 && tid == 0 && hk == 0 && rt == 0 && p.plan) p.plan[b] = make_int2(s_red[2], splits);
+    if (split == 0 && tid == 0 && hk == 0 && rt == 0 && p.plan) p.plan[b] = make_int2(first_slot, splits);
   }
   const int len = kv_length(p.c, p.lengths, b), n_tok = kv_count(p.counts, p.tokens, b);
 
@@ -257,7 +270,8 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attention_kv_split_kernel
   for (; tile < tile1; tile += kSplitWarps) {
     ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(bars + stage * 8, phase, nullptr));
     if (!ok) break;
-    const uint32_t ks = ring + stage * kSplitStageBytes, vs = ks + KT * D;
+    const uint8_t* ks = smem + (warp * kSplitStages + stage) * kSplitStageBytes;
+    const uint8_t* vs = ks + KT * D;
     // S = Q K^T
     float x[kTiles][4];
 #pragma unroll
@@ -265,7 +279,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attention_kv_split_kernel
       x[t][0] = x[t][1] = x[t][2] = x[t][3] = 0.0f;
 #pragma unroll
       for (int v = 0; v < D / 64; ++v) {
-        uint4 w = ld_shared_v4(ks + (8 * t + k_row) * D + 64 * v + 16 * c);
+        const uint4 w = *reinterpret_cast<const uint4*>(ks + (8 * t + k_row) * D + 64 * v + 16 * c);
         const uint32_t ww[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
 #pragma unroll
         for (int s = 0; s < 4; ++s)
@@ -345,11 +359,12 @@ __global__ void __launch_bounds__(32 * kSplitWarps, 2) attention_kv_split_kernel
       uint32_t w[4][D / 32];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const uint32_t at = vs + (16 * s + c + 4 * k) * D + (D / 8) * r;
+        const uint8_t* at = vs + (16 * s + c + 4 * k) * D + (D / 8) * r;
         if (D == 64) {
-          asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[k][0]), "=r"(w[k][1]) : "r"(at) : "memory");
+          const uint2 q2 = *reinterpret_cast<const uint2*>(at);
+          w[k][0] = q2.x, w[k][1] = q2.y;
         } else {
-          const uint4 q4 = ld_shared_v4(at);
+          const uint4 q4 = *reinterpret_cast<const uint4*>(at);
           w[k][0] = q4.x, w[k][1] = q4.y, w[k][D / 32 - 2] = q4.z, w[k][D / 32 - 1] = q4.w;
         }
       }
@@ -477,23 +492,40 @@ __global__ void __launch_bounds__(128) attention_kv_join_kernel(const KvAttnPara
   if (n <= 1) return;       // written by the block itself
   const float* src = p.part + at * (D + 4);
   step *= D + 4;
-  float m = -INFINITY, l = 0.0f, o[D / 32] = {};
-  for (int s = 0; s < n; ++s, src += step) {
-    const float2 ml = *reinterpret_cast<const float2*>(src + D);
-    const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.0f : m_new;
-    const float a = ex2_approx(m - ref), f = ex2_approx(ml.x - ref);
-    m = m_new;
-    l = l * a + ml.y * f;
+  // the parts' maxima and sums a lane each, then the parts four at a time
+  float m = -INFINITY;
+  for (int s = lane; s < n; s += 32) m = fmaxf(m, src[s * step + D]);
+  m = warp_max(m);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f, o[D / 32] = {};
+  for (int s0 = 0; s0 < n; s0 += 32) {
+    float f = 0.0f;
+    if (s0 + lane < n) {
+      const float2 ml = *reinterpret_cast<const float2*>(src + (s0 + lane) * step + D);
+      f = ex2_approx(ml.x - ref);
+      l = __fmaf_rn(ml.y, f, l);
+    }
+    const int end = min(32, n - s0);
+#pragma unroll 4
+    for (int s = 0; s < end; ++s) {
+      const float fs = __shfl_sync(0xffffffffu, f, s);
+      const float* v = src + (s0 + s) * step + lane * (D / 32);
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) o[k] = o[k] * a + src[lane * (D / 32) + k] * f;
+      for (int k = 0; k < D / 32; k += 2) {
+        const float2 x = *reinterpret_cast<const float2*>(v + k);
+        o[k] = __fmaf_rn(x.x, fs, o[k]);
+        o[k + 1] = __fmaf_rn(x.y, fs, o[k + 1]);
+      }
+    }
   }
+  l = warp_sum(l);
   const float f = l == 0.0f ? 0.0f : __frcp_rn(l);
   T* out = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1] + t * p.os[2] + lane * (D / 32);
 #pragma unroll
   for (int k = 0; k < D / 32; ++k) from_f32(o[k] * f, out[k]);
   if (p.lse && lane == 0)
     p.lse[(static_cast<int64_t>(b) * p.q_heads + h) * p.tokens + t] =
-        l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) + log2f(l)) * kLn2;
+        l == 0.0f ? -INFINITY : (ref + log2f(l)) * kLn2;
 }
 
 }  // namespace h3b

@@ -8,11 +8,11 @@
 // of fp16) stay in registers between the maximum and the quantisation, so every
 // input is read once and every code written once.  Bound: HBM, 2 B read and
 // 1 B written per element.
+#include <cstring>
+
 #include "kv_common.cuh"
 
 namespace h3b {
-
-constexpr int kKvThreads = 128;
 
 struct KvWriteParams {
   KvView c;
@@ -24,11 +24,61 @@ struct KvWriteParams {
   bool vec[2];             // rows can be read 16 bytes at a time
 };
 
-// VPT: vectors of 8 elements per thread = page * dim / 1024.
-template <typename T, int VPT>
-__global__ void __launch_bounds__(kKvThreads) kv_write_kernel(const KvWriteParams p) {
-  __shared__ float s_max[kKvThreads / 32];
-  __shared__ int s_sum[kKvThreads / 32][128];
+// Eight elements as they are in memory, and the largest magnitude among them:
+// for the 16-bit types on the bits (sign cleared, the order of the floats is the
+// order of the integers, infinities and NaN above all finite values).
+template <typename T> struct KvRaw {
+  uint32_t w[KvVec8<T>::kWords];
+  __device__ __forceinline__ void load(const T* p, bool vec) {
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < KvVec8<T>::kWords / 4; ++i) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+      }
+    } else {
+      T e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = p[i];
+      memcpy(w, e, sizeof(w));
+    }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < KvVec8<T>::kWords; ++i) w[i] = 0u;
+  }
+  __device__ __forceinline__ void values(float (&x)[8]) const {
+    T e[8];
+    memcpy(e, w, sizeof(w));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f32(e[i]);
+  }
+  __device__ __forceinline__ uint32_t top(uint32_t most) const {
+    if (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < KvVec8<T>::kWords; ++i) most = max(most, w[i] & 0x7fffffffu);
+    } else {
+#pragma unroll
+      for (int i = 0; i < KvVec8<T>::kWords; ++i) most = __vmaxu2(most, w[i] & 0x7fff7fffu);
+    }
+    return most;
+  }
+  // The magnitude as fp32 bits; anything above 0x7f7fffff stands for an infinity or a NaN.
+  static __device__ __forceinline__ uint32_t top_f32(uint32_t most) {
+    if (sizeof(T) == 4) return most;
+    const uint16_t m = static_cast<uint16_t>(max(most & 0xffffu, most >> 16));
+    T v;
+    memcpy(&v, &m, 2);
+    return __float_as_uint(to_f32(v));
+  }
+};
+
+// VPT: vectors of 8 elements per thread = page * dim / 8 / threads.
+template <typename T, int VPT, int kThreads>
+__global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvWriteParams p) {
+  constexpr int kWarps = kThreads / 32;
+  __shared__ uint32_t s_max[kWarps];
+  __shared__ int s_sum[kWarps][128];
   const int kv = blockIdx.x & 1, head = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const int count = p.counts ? min(p.counts[b], p.tokens) : p.tokens;
   const int start = p.start[b];
@@ -42,59 +92,55 @@ __global__ void __launch_bounds__(kKvThreads) kv_write_kernel(const KvWriteParam
   const int lo = static_cast<int>(max(static_cast<int64_t>(start), page_begin) - page_begin);   // first new row
   const int hi = static_cast<int>(min(end - page_begin, static_cast<int64_t>(p.c.page)));       // past the last one
   if (hi <= lo) return;
+
+  // the new rows are asked for before the page is looked up
+  const int chunk_shift = p.dim == 64 ? 3 : 4;
+  const T* src = static_cast<const T*>(p.x[kv]) + b * p.stride[kv][0] + head * p.stride[kv][1] +
+                 (page_begin - start) * p.stride[kv][2];
+  KvRaw<T> x[VPT];
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int i = tid + j * kThreads, row = i >> chunk_shift, col = (i & ((1 << chunk_shift) - 1)) * 8;
+    if (row >= lo && row < hi) x[j].load(src + row * p.stride[kv][2] + col, p.vec[kv]);
+    else x[j].zero();
+  }
   const int page = kv_page(p.c, b, slot);
   if (page < 0) return;
-
-  const int chunks = p.dim >> 3;
   const int64_t ph = static_cast<int64_t>(page) * p.c.heads + head;
   int8_t* codes = p.c.code[kv] + ph * p.c.page * p.dim;
   float* scale_at = p.c.scale[kv] + ph;
-  const T* src = static_cast<const T*>(p.x[kv]) + b * p.stride[kv][0] + head * p.stride[kv][1];
-  const int64_t row0 = page_begin - start;   // token of the page's row 0
-  const float old_scale = *scale_at;
+  const float old_scale = lo > 0 ? *scale_at : 0.0f;
 
-  // the new rows, and the largest magnitude among them (NaN and infinities give NaN or +inf)
-  float x[VPT][8];
-  float top = 0.0f;
-  bool bad = false;
+  uint32_t most = 0;
 #pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    const int i = tid + j * kKvThreads, row = i / chunks, col = (i % chunks) * 8;
-    if (row >= lo && row < hi) {
-      load8(src + (row0 + row) * p.stride[kv][2] + col, p.vec[kv], x[j]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        top = fmaxf(top, fabsf(x[j][e]));
-        bad |= !(fabsf(x[j][e]) <= 3.4028235e38f);
-      }
-    }
-  }
-  if (bad) top = INFINITY;
-  top = warp_max(top);
-  if ((tid & 31) == 0) s_max[tid >> 5] = top;
+  for (int j = 0; j < VPT; ++j) most = x[j].top(most);
+  most = __reduce_max_sync(0xffffffffu, KvRaw<T>::top_f32(most));
+  if ((tid & 31) == 0) s_max[tid >> 5] = most;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kKvThreads / 32; ++w) top = fmaxf(top, s_max[w]);
+  for (int w = 0; w < kWarps; ++w) most = max(most, s_max[w]);
 
-  float s = fmaxf(__fmul_rn(top, kKvInv127), kKvMinScale);
-  if (lo > 0) s = old_scale > s ? old_scale : s;
-  const bool lost = top == INFINITY || (lo > 0 && isnan(old_scale));
+  const bool lost = most > 0x7f7fffffu || isnan(old_scale);    // a NaN or an infinity, now or before
+  float s = fmaxf(__fmul_rn(__uint_as_float(most), kKvInv127), kKvMinScale);
+  s = old_scale > s ? old_scale : s;
   const bool grown = lo > 0 && s > old_scale;
   const bool complete = kv == 0 && hi == p.c.page;
   const float inv = __frcp_rn(s), ratio = __fdiv_rn(old_scale, s);
   int sum[8] = {};
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
-    const int i = tid + j * kKvThreads, row = i / chunks, col = (i % chunks) * 8;
-    uint2* at = reinterpret_cast<uint2*>(codes + row * p.dim + col);
+    const int i = tid + j * kThreads, row = i >> chunk_shift;
+    uint2* at = reinterpret_cast<uint2*>(codes) + i;
     uint2 w = make_uint2(0u, 0u);
     bool store = false;
     if (row >= lo && row < hi) {
       store = true;
       if (!lost) {   // |x * inv| <= 127 * (1 + 2^-22): no clamp is needed after rounding
+        float f[8];
+        x[j].values(f);
         uint32_t q[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) q[e] = rint_bits(__fmul_rn(x[j][e], inv));
+        for (int e = 0; e < 8; ++e) q[e] = rint_bits(__fmul_rn(f[e], inv));
         w = make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
       }
     } else if (row < lo && (grown || complete)) {
@@ -118,7 +164,8 @@ __global__ void __launch_bounds__(kKvThreads) kv_write_kernel(const KvWriteParam
   }
   if (tid == 0) *scale_at = lost ? __int_as_float(0x7fffffff) : s;
   if (complete) {
-    // a thread's vectors share their column (kKvThreads is a multiple of `chunks`)
+    // a thread's vectors share their column (the thread count is a multiple of the vectors in a row)
+    const int chunks = 1 << chunk_shift;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       for (int o = chunks; o < 32; o <<= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
@@ -130,7 +177,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_write_kernel(const KvWriteParam
     if (tid < p.dim) {
       int t = 0;
 #pragma unroll
-      for (int w = 0; w < kKvThreads / 32; ++w) t += s_sum[w][tid];
+      for (int w = 0; w < kWarps; ++w) t += s_sum[w][tid];
       p.c.k_sum[ph * p.dim + tid] = static_cast<int16_t>(t);
     }
   }
@@ -187,11 +234,11 @@ namespace {
 template <typename T>
 void launch_kv_write(const h3b::KvWriteParams& p, dim3 grid, cudaStream_t st) {
   switch (p.c.page * p.dim / 1024) {
-    case 1: h3b::kv_write_kernel<T, 1><<<grid, h3b::kKvThreads, 0, st>>>(p); break;
-    case 2: h3b::kv_write_kernel<T, 2><<<grid, h3b::kKvThreads, 0, st>>>(p); break;
-    case 4: h3b::kv_write_kernel<T, 4><<<grid, h3b::kKvThreads, 0, st>>>(p); break;
-    case 8: h3b::kv_write_kernel<T, 8><<<grid, h3b::kKvThreads, 0, st>>>(p); break;
-    default: h3b::kv_write_kernel<T, 16><<<grid, h3b::kKvThreads, 0, st>>>(p); break;
+    case 1: h3b::kv_write_kernel<T, 1, 128><<<grid, 128, 0, st>>>(p); break;
+    case 2: h3b::kv_write_kernel<T, 2, 128><<<grid, 128, 0, st>>>(p); break;
+    case 4: h3b::kv_write_kernel<T, 4, 128><<<grid, 128, 0, st>>>(p); break;
+    case 8: h3b::kv_write_kernel<T, 4, 256><<<grid, 256, 0, st>>>(p); break;
+    default: h3b::kv_write_kernel<T, 8, 256><<<grid, 256, 0, st>>>(p); break;
   }
 }
 

@@ -9,8 +9,8 @@
 // ties (lower page first) are exact.
 //
 // Two kernels: scores (a thread per page, all rows of the sequence and head
-// from shared memory) and the selection (a block per row: a radix select of the
-// (n-1)-th largest key, then an ordered compaction).
+// from shared memory) and the selection (a block per row: the (n-1)-th largest
+// key by bisection, then an ordered compaction).
 #include "kv_common.cuh"
 
 namespace h3b {
@@ -38,7 +38,7 @@ __device__ __forceinline__ int kv_last_page(const KvSelectParams& p, int b, int 
   return t >= n || pos < 0 ? -1 : pos >> p.c.page_shift;
 }
 
-constexpr int kSelThreads = 256;
+constexpr int kSelThreads = 128;
 constexpr int kSelRows = 64;     // query rows held in shared memory at once
 
 template <typename T, int D>
@@ -61,6 +61,7 @@ __global__ void __launch_bounds__(kSelThreads) kv_score_kernel(const KvSelectPar
       k[4 * i] = w.x, k[4 * i + 1] = w.y, k[4 * i + 2] = w.z, k[4 * i + 3] = w.w;
     }
   }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int per = max(1, kSelRows / p.group);      // query tokens per round
   float best = 0.0f;
   for (int t0 = 0; t0 < p.tokens; t0 += per) {
@@ -111,72 +112,113 @@ __global__ void __launch_bounds__(kSelThreads) kv_score_kernel(const KvSelectPar
   }
 }
 
-__global__ void __launch_bounds__(kSelThreads) kv_pick_kernel(const KvSelectParams p) {
-  __shared__ int s_hist[256];
-  __shared__ int s_scan[kSelThreads / 32][2];
-  __shared__ int s_pick[2];
+// The n - 1 best of a row's `last` keys, by bisection on the key's bits: the
+// threshold is built from the top bit down, counting the keys at or above it,
+// and found as soon as that count is right.  Each thread holds kPer consecutive
+// keys in registers; more pages than the block holds are read again each round.
+// (A histogram of 8-bit digits met 2047 keys in a few bins and took 22 us a row;
+// this takes 2 to 3.)
+constexpr int kPickThreads = 256;
+
+template <int kPer>
+__global__ void __launch_bounds__(kPickThreads) kv_pick_kernel(const KvSelectParams p) {
+  constexpr int kWarps = kPickThreads / 32;
+  __shared__ int s_count[2][kWarps];
   const int t = blockIdx.x, head = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t row = (static_cast<int64_t>(b) * p.c.heads + head) * p.tokens + t;
   int32_t* out = p.selected + row * p.n;
   const uint32_t* keys = p.keys + row * p.c.width;
   const int last = kv_last_page(p, b, t);
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // the scores; every block waits, so that none outlive this call
   if (last < p.n) {   // every page fits
-    for (int i = tid; i < p.n; i += kSelThreads) out[i] = i <= last ? i : -1;
+    for (int i = tid; i < p.n; i += kPickThreads) out[i] = i <= last ? i : -1;
     return;
   }
   const int want = p.n - 1;
-  if (want == 0) {
-    if (tid == 0) out[0] = last;
-    return;
-  }
-  // radix select: the want-th largest key, 8 bits a pass
-  uint32_t prefix = 0, mask = 0;
-  int left = want;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    s_hist[tid] = 0;
-    __syncthreads();
-    for (int i = tid; i < last; i += kSelThreads) {
-      const uint32_t k = keys[i];
-      if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & 255u], 1);
-    }
-    __syncthreads();
-    if (tid == 0) {
-      int above = 0, d = 255;
-      while (d > 0 && above + s_hist[d] < left) above += s_hist[d--];
-      s_pick[0] = d;
-      s_pick[1] = left - above;
-    }
-    __syncthreads();
-    prefix |= static_cast<uint32_t>(s_pick[0]) << shift;
-    mask |= 255u << shift;
-    left = s_pick[1];
-  }
-  // keys above the threshold, and the first `left` that equal it, in page order
-  int n_out = 0, n_tie = 0;
-  for (int i0 = 0; i0 < last; i0 += kSelThreads) {
-    const int i = i0 + tid;
-    const uint32_t k = i < last ? keys[i] : 0u;
-    const bool tie = i < last && k == prefix, above = i < last && k > prefix;
-    const unsigned mt = __ballot_sync(0xffffffffu, tie), ma = __ballot_sync(0xffffffffu, above);
-    if (lane == 0) {
-      s_scan[warp][0] = __popc(mt);
-      s_scan[warp][1] = __popc(ma);
-    }
-    __syncthreads();
-    int ties = n_tie, aboves = 0, all_t = 0, all_a = 0;
-    for (int w = 0; w < kSelThreads / 32; ++w) {
-      if (w < warp) ties += s_scan[w][0], aboves += s_scan[w][1];
-      all_t += s_scan[w][0];
-      all_a += s_scan[w][1];
-    }
-    ties += __popc(mt & ((1u << lane) - 1u));        // ties before this page
-    aboves += __popc(ma & ((1u << lane) - 1u));
-    if (above || (tie && ties < left)) out[n_out + aboves + min(ties, left) - min(n_tie, left)] = i;
-    n_out += all_a + min(n_tie + all_t, left) - min(n_tie, left);
-    n_tie += all_t;
-    __syncthreads();
-  }
   if (tid == 0) out[want] = last;
+  if (want == 0) return;
+  const int rounds = (last + kPickThreads * kPer - 1) / (kPickThreads * kPer);
+  uint32_t k[kPer];
+  auto load = [&](int round) {
+    const int i0 = (round * kPickThreads + tid) * kPer;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) k[e] = i0 + e < last ? __ldcg(keys + i0 + e) : 0u;
+  };
+  if (rounds == 1) load(0);
+  // largest threshold with at least `want` keys at or above it (keys are never 0 but on bad pages)
+  uint32_t thr = 0;
+  int at_least = last;
+  for (int bit = 31; bit >= 0 && at_least != want; --bit) {
+    const uint32_t cand = thr | (1u << bit);
+    int n = 0;
+    for (int r = 0; r < rounds; ++r) {
+      if (rounds > 1) load(r);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) n += k[e] >= cand ? 1 : 0;
+    }
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) s_count[bit & 1][warp] = n;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) n += s_count[bit & 1][w];
+    if (n >= want) {
+      thr = cand;
+      at_least = n;
+    }
+  }
+  // keys above the threshold, and of those that equal it the first in page order
+  int above = 0;
+  if (at_least != want) {
+    for (int r = 0; r < rounds; ++r) {
+      if (rounds > 1) load(r);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) above += k[e] > thr ? 1 : 0;
+    }
+    above = __reduce_add_sync(0xffffffffu, above);
+    __syncthreads();
+    if (lane == 0) s_count[0][warp] = above;
+    __syncthreads();
+    above = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) above += s_count[0][w];
+  }
+  const int ties = at_least != want ? want - above : last;    // that are taken
+  int n_out = 0, n_tie = 0;
+  for (int r = 0; r < rounds; ++r) {
+    if (rounds > 1) load(r);
+    const int i0 = (r * kPickThreads + tid) * kPer;
+    int mine = 0;                                             // above << 16 | equal
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      if (i0 + e < last) mine += k[e] > thr ? 1 << 16 : k[e] == thr ? 1 : 0;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    __syncthreads();
+    if (lane == 31) s_count[1][warp] = incl;
+    __syncthreads();
+    int before = incl - mine, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      before += w < warp ? s_count[1][w] : 0;
+      all += s_count[1][w];
+    }
+    int tie = n_tie + (before & 0xffff);
+    int at = n_out + (before >> 16) + min(tie, ties) - min(n_tie, ties);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      if (i0 + e >= last) continue;
+      const bool equal = k[e] == thr;
+      if (k[e] > thr || (equal && tie < ties)) out[at++] = i0 + e;
+      tie += equal ? 1 : 0;
+    }
+    n_out += (all >> 16) + min(n_tie + (all & 0xffff), ties) - min(n_tie, ties);
+    n_tie += all & 0xffff;
+  }
 }
 
 }  // namespace h3b
@@ -228,6 +270,17 @@ extern "C" int h3b_kv_select_i8(const void* q, const int64_t* q_strides, const h
   }
   rc = h3b_host::check_launch(name);
   if (rc) return rc;
-  h3b::kv_pick_kernel<<<g2, h3b::kSelThreads, 0, st>>>(p);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = g2;
+  cfg.blockDim = dim3(h3b::kPickThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};   // its blocks may be resident before the scores are done; they wait for them
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = table_width <= 4 * h3b::kPickThreads ? cudaLaunchKernelEx(&cfg, h3b::kv_pick_kernel<4>, p)
+                                                       : cudaLaunchKernelEx(&cfg, h3b::kv_pick_kernel<16>, p);
+  if (e != cudaSuccess) return h3b_host::set_error(H3B_ECUDA, "%s: selection launch: %s", name, cudaGetErrorString(e));
   return h3b_host::check_launch(name);
 }

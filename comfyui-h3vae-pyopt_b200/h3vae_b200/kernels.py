@@ -7,6 +7,8 @@ These are the only functions in the package that touch the native library.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -42,6 +44,20 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+# The current stream's handle without building a Stream object (2 us less a call), where torch has the call.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _kv_stream(device: torch.device) -> int:
+    return _stream(device) if _raw_stream is None or device.index is None else _raw_stream(device.index)
+
+
+@functools.lru_cache(maxsize=256)
+def _kv_workspace_bytes(name: str, *sizes: int) -> int:
+    """Bytes that the library's `name`_workspace_size asks for (a function of sizes alone)."""
+    return int(getattr(_lib.load(), name + "_workspace_size")(*sizes))
 
 
 def _require_cuda(*tensors: torch.Tensor | None) -> torch.device:
@@ -797,7 +813,7 @@ def kv_write_i8(cache, page_table: torch.Tensor, start: torch.Tensor, k: torch.T
     _lib.check(_lib.load().h3b_kv_write_i8(
         cache.struct, table, batch, width, _kv_index(start, "start", (batch,), dev),
         _kv_index(counts, "counts", (batch,), dev), k.data_ptr(), _strides3(k), v.data_ptr(), _strides3(v), k.shape[2],
-        _KV_TYPES[k.dtype], _stream(dev)))
+        _KV_TYPES[k.dtype], _kv_stream(dev)))
     _count(1)
 
 
@@ -817,7 +833,7 @@ def kv_read_i8(cache, page_table: torch.Tensor, lengths: torch.Tensor, tokens: i
         _lib.check(_lib.load().h3b_kv_read_i8(
             cache.struct, table, batch, width, _kv_index(start, "start", (batch,), dev),
             _kv_index(lengths, "lengths", (batch,), dev), k.data_ptr(), v.data_ptr(), tokens, _KV_TYPES[dtype],
-            _stream(dev)))
+            _kv_stream(dev)))
         _count(1)
     return k, v
 
@@ -860,14 +876,14 @@ def attention_kv_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: t
     lse = torch.empty((batch, heads, tokens), device=dev, dtype=F32) if return_lse else None
     if tokens:
         lib = _lib.load()
-        ws_bytes = lib.h3b_attention_kv_i8_workspace_size(batch, heads, cache.kv_heads, tokens, dim, width,
-                                                          cache.page_size, n_sel)
+        ws_bytes = _kv_workspace_bytes("h3b_attention_kv_i8", batch, heads, cache.kv_heads, tokens, dim, width,
+                                       cache.page_size, n_sel)
         ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
         _lib.check(lib.h3b_attention_kv_i8(
             q.data_ptr(), _strides3(q), cache.struct, table, batch, width, _kv_index(lengths, "lengths", (batch,), dev),
             _kv_index(counts, "counts", (batch,), dev), heads, tokens, float(scale), 1 if causal else 0, window,
             _ptr(selected), n_sel, _KV_TYPES[q.dtype], out.data_ptr(), _strides3(out), _ptr(lse), ws.data_ptr(),
-            ws_bytes, _stream(dev)))
+            ws_bytes, _kv_stream(dev)))
         _count(1)
     return (out, lse) if return_lse else out
 
@@ -885,11 +901,11 @@ def kv_select_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torc
     selected = torch.empty((batch, cache.kv_heads, tokens, pages), device=dev, dtype=_I32)
     if tokens:
         lib = _lib.load()
-        ws_bytes = lib.h3b_kv_select_i8_workspace_size(batch, cache.kv_heads, tokens, width)
+        ws_bytes = _kv_workspace_bytes("h3b_kv_select_i8", batch, cache.kv_heads, tokens, width)
         ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
         _lib.check(lib.h3b_kv_select_i8(
             q.data_ptr(), _strides3(q), cache.struct, table, batch, width, _kv_index(lengths, "lengths", (batch,), dev),
             _kv_index(counts, "counts", (batch,), dev), heads, tokens, pages, _KV_TYPES[q.dtype], selected.data_ptr(),
-            ws.data_ptr(), ws_bytes, _stream(dev)))
+            ws.data_ptr(), ws_bytes, _kv_stream(dev)))
         _count(2)
     return selected
