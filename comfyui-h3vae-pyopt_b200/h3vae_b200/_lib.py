@@ -94,20 +94,18 @@ class KvCacheStruct(ctypes.Structure):
                 ("num_pages", c_int64), ("kv_heads", c_int64), ("page_size", c_int64), ("head_dim", c_int64)]
 
 
-_kvp = POINTER(KvCacheStruct)
-
-# include/h3vae_b200_kv.h: the paged INT8 key/value cache
+# include/h3vae_b200_kv.h: the paged INT8 key/value cache (the struct by address; strides as three packed int64)
 _KV_SIGNATURES = {
-    "h3b_kv_write_i8": (c_int, [_kvp, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, _i64p, c_void_p, _i64p,
+    "h3b_kv_write_i8": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                 c_int64, c_int, c_void_p]),
-    "h3b_kv_read_i8": (c_int, [_kvp, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,
+    "h3b_kv_read_i8": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,
                                c_void_p]),
     "h3b_attention_kv_i8_workspace_size": (c_size_t, [c_int64] * 8),
-    "h3b_attention_kv_i8": (c_int, [c_void_p, _i64p, _kvp, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64,
-                                    c_int64, c_float, c_int, c_int64, c_void_p, c_int64, c_int, c_void_p, _i64p,
+    "h3b_attention_kv_i8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64,
+                                    c_int64, c_float, c_int, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p,
                                     c_void_p, c_void_p, c_size_t, c_void_p]),
     "h3b_kv_select_i8_workspace_size": (c_size_t, [c_int64] * 4),
-    "h3b_kv_select_i8": (c_int, [c_void_p, _i64p, _kvp, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64,
+    "h3b_kv_select_i8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64,
                                  c_int64, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
 }
 
@@ -160,9 +158,6 @@ def check(rc: int) -> None:
 def i64_array(values) -> ctypes.Array:
     vals = [int(v) for v in values]
     return (c_int64 * len(vals))(*vals)
-
-
-i64_x3 = c_int64 * 3
 
 
 def device_error(clear: bool = True) -> int:

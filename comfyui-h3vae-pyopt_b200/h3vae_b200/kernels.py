@@ -8,6 +8,7 @@ These are the only functions in the package that touch the native library.
 from __future__ import annotations
 
 import functools
+import struct
 
 import torch
 
@@ -761,6 +762,9 @@ def attention_f16(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: floa
 # Paged INT8 key/value cache (h3vae_b200.kv_cache.KVCacheI8)
 # ---------------------------------------------------------------------------
 _KV_TYPES = {F16: 0, torch.bfloat16: 1, F32: 2}
+_KV_ROWS = (F16, torch.bfloat16, F32)
+_KV_QUERIES = (F16, torch.bfloat16)
+_pack3 = struct.Struct("3q").pack
 _I32 = torch.int32
 
 
@@ -768,7 +772,7 @@ def _kv_index(t: torch.Tensor | None, name: str, shape: tuple, dev: torch.device
     """Data pointer of a contiguous int32 tensor of `shape` on `dev` (None passes)."""
     if t is None:
         return None
-    if t.dtype != _I32 or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype != _I32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
     if t.device != dev:
         raise ValueError(f"{name} must be on the cache's device")
@@ -778,20 +782,21 @@ def _kv_index(t: torch.Tensor | None, name: str, shape: tuple, dev: torch.device
 def _kv_table(cache, page_table: torch.Tensor) -> tuple[int, int, int]:
     if page_table.ndim != 2:
         raise ValueError("page_table must be int32 [batch, pages]")
-    batch, width = page_table.shape
-    return _kv_index(page_table, "page_table", (batch, width), cache.device), batch, width
+    batch, width = shape = page_table.shape
+    return _kv_index(page_table, "page_table", shape, cache.device), batch, width
 
 
-def _kv_rows(t: torch.Tensor, name: str, types: tuple, cache) -> None:
+def _kv_rows(t: torch.Tensor, name: str, types: tuple, cache) -> bytes:
+    """Checks [batch, heads, tokens, head_dim] rows; returns their batch, head and token strides as the library
+    takes them (three int64)."""
     if t.device != cache.device:
         raise ValueError(f"{name} must be on the cache's device")
-    if t.ndim != 4 or t.dtype not in types or t.shape[3] != cache.head_dim or (t.stride(3) != 1 and t.numel()):
-        raise ValueError(f"{name} must be [batch, heads, tokens, {cache.head_dim}] with unit dim stride, one of {types}")
-
-
-def _strides3(t: torch.Tensor):
-    s = t.stride()
-    return _lib.i64_x3(s[0], s[1], s[2])
+    if t.ndim != 4 or t.dtype not in types:
+        raise ValueError(f"{name} must be [batch, heads, tokens, {cache.head_dim}], one of {types}")
+    s0, s1, s2, s3 = t.stride()
+    if t.shape[3] != cache.head_dim or (s3 != 1 and t.numel()):
+        raise ValueError(f"{name} must be [batch, heads, tokens, {cache.head_dim}] with unit dim stride")
+    return _pack3(s0, s1, s2)
 
 
 def kv_write_i8(cache, page_table: torch.Tensor, start: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
@@ -801,8 +806,8 @@ def kv_write_i8(cache, page_table: torch.Tensor, start: torch.Tensor, k: torch.T
     a page that already holds earlier tokens keeps the larger scale and requantises them when it grew.
     page_table int32 [B, pages], start and counts int32 [B]."""
     table, batch, width = _kv_table(cache, page_table)
-    _kv_rows(k, "k", (F16, torch.bfloat16, F32), cache)
-    _kv_rows(v, "v", (k.dtype,), cache)
+    k_strides = _kv_rows(k, "k", _KV_ROWS, cache)
+    v_strides = _kv_rows(v, "v", (k.dtype,), cache)
     if k.shape != v.shape or k.shape[0] != batch or k.shape[1] != cache.kv_heads:
         raise ValueError(f"k and v must both be [{batch}, {cache.kv_heads}, tokens, {cache.head_dim}]")
     if start is None:
@@ -812,7 +817,7 @@ def kv_write_i8(cache, page_table: torch.Tensor, start: torch.Tensor, k: torch.T
         return
     _lib.check(_lib.load().h3b_kv_write_i8(
         cache.struct, table, batch, width, _kv_index(start, "start", (batch,), dev),
-        _kv_index(counts, "counts", (batch,), dev), k.data_ptr(), _strides3(k), v.data_ptr(), _strides3(v), k.shape[2],
+        _kv_index(counts, "counts", (batch,), dev), k.data_ptr(), k_strides, v.data_ptr(), v_strides, k.shape[2],
         _KV_TYPES[k.dtype], _kv_stream(dev)))
     _count(1)
 
@@ -838,11 +843,12 @@ def kv_read_i8(cache, page_table: torch.Tensor, lengths: torch.Tensor, tokens: i
     return k, v
 
 
-def _kv_query(q: torch.Tensor, cache, batch: int) -> tuple[int, int]:
-    _kv_rows(q, "q", (F16, torch.bfloat16), cache)
-    if q.shape[0] != batch or q.shape[1] == 0 or q.shape[1] % cache.kv_heads:
+def _kv_query(q: torch.Tensor, cache, batch: int) -> tuple[int, int, bytes]:
+    strides = _kv_rows(q, "q", _KV_QUERIES, cache)
+    b, heads, tokens, _ = q.shape
+    if b != batch or heads == 0 or heads % cache.kv_heads:
         raise ValueError(f"q must be [{batch}, a multiple of {cache.kv_heads} heads, tokens, {cache.head_dim}]")
-    return q.shape[1], q.shape[2]
+    return heads, tokens, strides
 
 
 def attention_kv_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.Tensor, scale: float, *,
@@ -859,12 +865,16 @@ def attention_kv_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: t
     Writes `out` (default: a new [B, T, Hq, D] tensor, returned as its [B, Hq, T, D] view); with return_lse also
     returns the natural log of each row's sum of exponentials, fp32 [B, Hq, T]."""
     table, batch, width = _kv_table(cache, page_table)
-    heads, tokens = _kv_query(q, cache, batch)
+    heads, tokens, q_strides = _kv_query(q, cache, batch)
     dev, dim = cache.device, cache.head_dim
     if out is None:
-        out = torch.empty((batch, tokens, heads, dim), device=dev, dtype=q.dtype).transpose(1, 2)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(3) != 1:
-        raise ValueError("out must have q's shape, dtype and device, and unit dim stride")
+        strides = (tokens * heads * dim, dim, heads * dim, 1)
+        out = torch.empty_strided((batch, heads, tokens, dim), strides, device=dev, dtype=q.dtype)
+        out_strides = _pack3(*strides[:3])
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out must have q's shape and dtype")
+    else:
+        out_strides = _kv_rows(out, "out", _KV_QUERIES, cache)
     if lengths is None:
         raise ValueError("lengths must be int32 [batch]")
     n_sel = 0
@@ -880,9 +890,9 @@ def attention_kv_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: t
                                        cache.page_size, n_sel)
         ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
         _lib.check(lib.h3b_attention_kv_i8(
-            q.data_ptr(), _strides3(q), cache.struct, table, batch, width, _kv_index(lengths, "lengths", (batch,), dev),
+            q.data_ptr(), q_strides, cache.struct, table, batch, width, _kv_index(lengths, "lengths", (batch,), dev),
             _kv_index(counts, "counts", (batch,), dev), heads, tokens, float(scale), 1 if causal else 0, window,
-            _ptr(selected), n_sel, _KV_TYPES[q.dtype], out.data_ptr(), _strides3(out), _ptr(lse), ws.data_ptr(),
+            _ptr(selected), n_sel, _KV_TYPES[q.dtype], out.data_ptr(), out_strides, _ptr(lse), ws.data_ptr(),
             ws_bytes, _kv_stream(dev)))
         _count(1)
     return (out, lse) if return_lse else out
@@ -894,7 +904,7 @@ def kv_select_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torc
     product with the row-quantised query (the maximum over the group's heads; ties: the lower page).
     q, lengths, counts as in attention_kv_i8; returns int32 [B, H, T, pages], ascending, -1 where none is left."""
     table, batch, width = _kv_table(cache, page_table)
-    heads, tokens = _kv_query(q, cache, batch)
+    heads, tokens, q_strides = _kv_query(q, cache, batch)
     dev = cache.device
     if pages < 1 or lengths is None:
         raise ValueError("pages must be at least 1 and lengths int32 [batch]")
@@ -904,7 +914,7 @@ def kv_select_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torc
         ws_bytes = _kv_workspace_bytes("h3b_kv_select_i8", batch, cache.kv_heads, tokens, width)
         ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
         _lib.check(lib.h3b_kv_select_i8(
-            q.data_ptr(), _strides3(q), cache.struct, table, batch, width, _kv_index(lengths, "lengths", (batch,), dev),
+            q.data_ptr(), q_strides, cache.struct, table, batch, width, _kv_index(lengths, "lengths", (batch,), dev),
             _kv_index(counts, "counts", (batch,), dev), heads, tokens, pages, _KV_TYPES[q.dtype], selected.data_ptr(),
             ws.data_ptr(), ws_bytes, _kv_stream(dev)))
         _count(2)

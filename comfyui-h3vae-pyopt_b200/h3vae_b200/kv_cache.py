@@ -23,7 +23,7 @@ class KVCacheI8:
     replaced for the life of the object."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "k_sum", "num_pages", "kv_heads", "page_size", "head_dim", "device",
-                 "struct")
+                 "struct", "_struct")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                  k_sum: torch.Tensor):
@@ -43,9 +43,9 @@ class KVCacheI8:
         self.k, self.v, self.k_scale, self.v_scale, self.k_sum = k, v, k_scale, v_scale, k_sum
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = pages, heads, page, dim
         self.device = k.device
-        self.struct = ctypes.pointer(_lib.KvCacheStruct(
-            k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k_sum.data_ptr(), pages, heads, page,
-            dim))
+        self._struct = _lib.KvCacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                          k_sum.data_ptr(), pages, heads, page, dim)
+        self.struct = ctypes.addressof(self._struct)     # what the library takes
 
     @classmethod
     def empty(cls, num_pages: int, kv_heads: int, head_dim: int = 64, page_size: int = 64,

@@ -1,6 +1,7 @@
 """What of the key/value cache needs no GPU: the library's exports and its refusals, which come before any launch."""
 import ctypes
 import re
+import struct
 
 from conftest import ROOT
 
@@ -22,13 +23,13 @@ def test_exports_match_the_header():
 def _cache(lib_mod, **kw):
     fields = dict(k=64, v=64, k_scale=64, v_scale=64, k_sum=64, num_pages=4, kv_heads=2, page_size=16, head_dim=64)
     fields.update(kw)
-    return ctypes.byref(lib_mod.KvCacheStruct(**fields))
+    return ctypes.byref(lib_mod.KvCacheStruct(**fields))      # kept alive by the reference
 
 
 def test_refusals_at_the_c_entries():
     """Pointers here are never followed: every call is refused on the host."""
     lib_mod, lib = _lib()
-    st = lib_mod.i64_x3(0, 0, 64)
+    st = struct.pack("3q", 0, 0, 64)
 
     def write(cache, table=64, batch=1, width=2, start=64, k=64, tokens=1, dtype=0):
         return lib.h3b_kv_write_i8(cache, table, batch, width, start, None, k, st, 64, st, tokens, dtype, None)
