@@ -32,6 +32,7 @@ struct KvAttnParams {
   float scale_log2;
   // split plan (see attention_kv_split_kernel)
   int row_tiles, slots, target, chunk;
+  int cluster;     // > 0: the slots of a row tile are one cluster, which joins them itself
   float* part;     // [slot, kv head, row tile, row] x (dim + 2): weighted codes, m, l
   int2* plan;      // per sequence: first slot, number of slots
 };

@@ -28,6 +28,7 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
 constexpr int kSplitWarps = 4;
 constexpr int kSplitStages = 2;
 constexpr int kSplitBlocks = 3;       // blocks an SM holds (two with three stages: 154 against 139 us on 16 x 32768 keys)
+constexpr int kSplitCluster = 8;      // most blocks that join through shared memory
 constexpr int kSplitRows = 16;
 constexpr int kSplitPages = 256;      // pages a block's run of tiles may span
 constexpr int kSplitStageBytes = 8192;
@@ -84,6 +85,15 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_s
     const int tiles = (p.n_selected * p.c.page + KT - 1) / KT;
     tile0 = min(split * p.chunk, tiles);
     tile1 = min(tile0 + p.chunk, tiles);
+  } else if (p.cluster) {
+    b = blockIdx.z;
+    rt = blockIdx.x / p.slots;
+    slot = split = blockIdx.x % p.slots;
+    splits = p.slots;
+    int t0;
+    const int tiles = split_tiles(p, b, KT, t0), chunk = (tiles + splits - 1) / splits;
+    tile0 = t0 + min(split * chunk, tiles);
+    tile1 = t0 + min(split * chunk + chunk, tiles);
   } else {
     rt = blockIdx.x / p.slots;
     slot = blockIdx.x % p.slots;
@@ -421,6 +431,22 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_s
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __syncthreads();
   const int rows = min(kOut, g_rows - rt * kSplitRows);
+  auto finish = [&](int row, int d, float4 acc, float m_row, float l_row) {   // dims d .. d + 3 of a joined row
+    const int full = rt * kSplitRows + row;
+    const int t = kSparse ? t_sparse : full / p.group, h = hk * p.group + (kSparse ? full : full % p.group);
+    const float f = l_row == 0.0f ? 0.0f : __frcp_rn(l_row);
+    T* out = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1] + t * p.os[2] + d;
+    from_f32(acc.x * f, out[0]);
+    from_f32(acc.y * f, out[1]);
+    from_f32(acc.z * f, out[2]);
+    from_f32(acc.w * f, out[3]);
+    if (p.lse && d == 0)
+      p.lse[(static_cast<int64_t>(b) * p.q_heads + h) * p.tokens + t] =
+          l_row == 0.0f ? -INFINITY : ((m_row == -INFINITY ? 0.0f : m_row) + log2f(l_row)) * kLn2;
+  };
+  constexpr int kRow = D + 4;                                        // weighted codes, m, l of a row of this block
+  float* s_c = s_ml + kSplitWarps * kOut * 2;
+  static_assert((kSplitWarps * kOut * (D + 6) + kOut * kRow) * 4 <= S::kRing, "join buffer");
   for (int i = tid; i < rows * (D / 4); i += kThreads) {
     const int row = i / (D / 4), d = (i % (D / 4)) * 4;
     float mm = -INFINITY;
@@ -439,27 +465,54 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_s
       acc.w = __fmaf_rn(f, v.w, acc.w);
       ll = __fmaf_rn(f, s_ml[(w * kOut + row) * 2 + 1], ll);
     }
-    const int full = rt * kSplitRows + row;
-    if (splits > 1) {
-      const int64_t at = ((static_cast<int64_t>(slot) * p.c.heads + hk) * p.row_tiles + rt) * kSplitRows + row;
-      *reinterpret_cast<float4*>(p.part + at * (D + 4) + d) = acc;
-      if (d == 0) *reinterpret_cast<float2*>(p.part + at * (D + 4) + D) = make_float2(mm, ll);
+    if (splits == 1) {
+      finish(row, d, acc, mm, ll);
     } else {
-      const int t = kSparse ? t_sparse : full / p.group, h = hk * p.group + (kSparse ? full : full % p.group);
-      const float f = ll == 0.0f ? 0.0f : __frcp_rn(ll);
-      T* out = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1] + t * p.os[2] + d;
-      from_f32(acc.x * f, out[0]);
-      from_f32(acc.y * f, out[1]);
-      from_f32(acc.z * f, out[2]);
-      from_f32(acc.w * f, out[3]);
-      if (p.lse && d == 0)
-        p.lse[(static_cast<int64_t>(b) * p.q_heads + h) * p.tokens + t] =
-            ll == 0.0f ? -INFINITY : (rf + log2f(ll)) * kLn2;
+      const int64_t at = ((static_cast<int64_t>(slot) * p.c.heads + hk) * p.row_tiles + rt) * kSplitRows + row;
+      float* dst = p.cluster ? s_c + row * kRow : p.part + at * kRow;
+      *reinterpret_cast<float4*>(dst + d) = acc;
+      if (d == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(mm, ll);
     }
+  }
+  if (p.cluster && splits > 1) {
+    // the cluster's blocks join their rows through each other's shared memory, a share of the dims each
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    const uint32_t mine = smem_u32(s_c);
+    for (int i = split * kThreads + tid; i < rows * (D / 4); i += splits * kThreads) {
+      const int row = i / (D / 4), d = (i % (D / 4)) * 4;
+      float mm = -INFINITY, ll = 0.0f;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float2 ml[kSplitCluster];
+      float4 v[kSplitCluster];
+#pragma unroll
+      for (int w = 0; w < kSplitCluster; ++w) {
+        if (w >= splits) break;
+        uint32_t at;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(mine + row * kRow * 4), "r"(w));
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml[w].x), "=f"(ml[w].y) : "r"(at + D * 4));
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v[w].x), "=f"(v[w].y), "=f"(v[w].z), "=f"(v[w].w)
+                     : "r"(at + d * 4));
+        mm = fmaxf(mm, ml[w].x);
+      }
+      const float rf = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+      for (int w = 0; w < kSplitCluster; ++w) {
+        if (w >= splits) break;
+        const float f = ex2_approx(ml[w].x - rf);
+        acc.x = __fmaf_rn(f, v[w].x, acc.x);
+        acc.y = __fmaf_rn(f, v[w].y, acc.y);
+        acc.z = __fmaf_rn(f, v[w].z, acc.z);
+        acc.w = __fmaf_rn(f, v[w].w, acc.w);
+        ll = __fmaf_rn(f, ml[w].y, ll);
+      }
+      finish(row, d, acc, mm, ll);
+    }
+    // no block leaves while another reads its shared memory
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
 }
 
-// Joins the slots of a row: one warp per row, D / 32 dims a lane.
 enum KvParts { kPartsPlan, kPartsSparse, kPartsTile };   // how the parts of a row are laid out
 
 template <typename T, int D, KvParts kParts>

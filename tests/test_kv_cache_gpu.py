@@ -547,3 +547,32 @@ def test_refusals(cuda_lib):
     K.kv_write_i8(cache, table, one, k[:, :, :0], k[:, :, :0])
     assert K.attention_kv_i8(q[:, :, :0], cache, table, one, 1.0).shape == (1, 4, 0, 64)
     assert K.kv_select_i8(q[:, :, :0], cache, table, one, 2).shape == (1, 2, 0, 2)
+
+
+def test_attention_over_many_selected_pages(cuda_lib):
+    """More pages than one cluster's blocks hold: the parts go through the workspace."""
+    from h3vae_b200 import kernels as K
+    rng = np.random.default_rng(13)
+    lens = [16 * 2600 + 5]
+    ref, rows, table = _filled(rng, lens, 1, 64, 16)
+    cache = _cache(ref)
+    q = torch.from_numpy(rng.standard_normal((1, 2, 2, 64)) * 2).half().cuda()
+    sel = K.kv_select_i8(q, cache, table, _i32(lens), 2300)
+    got = K.attention_kv_i8(q, cache, table, _i32(lens), 0.125, selected=sel)
+    out, _, bound = _attend_all(ref, rows, q, lens, [2], 0.125, 16, selected=sel.cpu().numpy())
+    R.check(got, out, bound, torch.float16)
+
+
+def test_long_single_streams(cuda_lib):
+    """One and three long streams of one head: more runs of keys than a cluster has blocks."""
+    from h3vae_b200 import kernels as K
+    rng = np.random.default_rng(14)
+    lens = [30000, 17, 9001]
+    ref, rows, table = _filled(rng, lens, 1, 128, 128)
+    cache = _cache(ref)
+    for t, group, pick in ((1, 1, [0]), (1, 10, [0, 1, 2]), (4, 1, [1, 2, 0])):
+        q = torch.from_numpy(rng.standard_normal((len(pick), group, t, 128)) * 2).to(torch.bfloat16).cuda()
+        n = [lens[i] for i in pick]
+        got = K.attention_kv_i8(q, cache, table[pick].contiguous(), _i32(n), 0.09)
+        out, _, bound = _attend_all(ref, [rows[i] for i in pick], q, n, [t] * len(pick), 0.09, 128)
+        R.check(got, out, bound, torch.bfloat16)
