@@ -70,6 +70,14 @@ __device__ __forceinline__ uint32_t codes_to_h2(uint32_t biased, uint32_t select
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 
+// Copies `bytes` (a multiple of 16, both addresses 16-byte aligned) to shared
+// memory; their arrival counts on the barrier.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
 // A query row as fp16.  bf16 rows are scaled by a power of two so that their
 // largest value lies in [1, 2): every value that matters at fp32 precision of
 // the product is then exact in fp16; `back` undoes the scaling.

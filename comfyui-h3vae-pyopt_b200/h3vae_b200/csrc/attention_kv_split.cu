@@ -41,12 +41,6 @@ struct KvSplit {
   static constexpr int kSmem = kRing + kMeta + kSplitWarps * kSplitStages * 8 + 128;
 };
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
-
 // Tiles a sequence's rows need, in tiles of `keys`.
 __device__ __forceinline__ int split_tiles(const KvAttnParams& p, int b, int keys, int& tile0) {
   const int len = kv_length(p.c, p.lengths, b), n = kv_count(p.counts, p.tokens, b);

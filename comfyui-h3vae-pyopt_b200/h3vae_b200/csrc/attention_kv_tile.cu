@@ -4,25 +4,25 @@
 // One CTA = one (sequence, kv head) and two tiles of 128 rows; a row is a
 // (query token, head of the group), so grouped heads share the keys a CTA
 // reads.  12 warps:
-//   warps 0..2   codes to operands: half tiles of 64 keys of K or V are read from
-//                their pages 16 codes at a time, converted to fp16 (exactly: codes are
+//   warps 0..2   codes to operands: half tiles of 64 keys of K or V come from their
+//                pages by bulk copies, are converted to fp16 (exactly: codes are
 //                whole numbers) and written to shared memory in the 128-byte
-//                swizzle the tensor core reads; tiles go through one ring in the
-//                order they are used: K0 K1 V0 K2 V1 K3 V2 ...  The block's scales,
-//                per 16 keys, go with K.
-//   warp 3       TMEM owner and MMA issuer: S(t) = Q(t) K^T, O(t) += W(t) V(t).
+//                swizzle the tensor core reads; tiles of 128 keys go through one
+//                ring, K0 V0 K1 V1 ...  The block's scales, per 16 keys, go with K.
+//   warp 3       TMEM owner and MMA issuer: S(t) = Q(t) K^T, O(t) += W(t) V, the two
+//                row tiles in turn, so that one's products run under the other's
+//                exponentials.
 //   warps 4..11  softmax, four per row tile, one row per thread (its TMEM lane):
-//                a row's 128 products come out of TMEM at once, which frees S for
-//                the next block; x = S * (ks * scale * log2 e) + log2 vs against
-//                the running maximum gives weights in fp16 for the second product
-//                and, times 1 / vs in fp32, the denominator.
-// The reference maximum is the first block's that a row sees; a later block is
-// taken against it as it is, and only when 16 of its weights sum to more than
-// 2^14 (fp16 holds 65504, and keeps its 11 bits up to there) is its own maximum
-// looked for, the block redone and O rescaled in TMEM.  The two row tiles take
-// turns on the SFU, so that one tile's exponentials overlap the other's products.
-// Blocks that no row of the CTA sees are not visited, and only blocks on an edge
-// of a row's range test each key.
+//                x = S * (ks * scale * log2 e) + log2 vs against the row's maximum
+//                gives weights and, times 1 / vs in fp32, the denominator.  The
+//                weights go back in fp16 over the products, and the second product
+//                takes them from there: shared memory, which both products and the
+//                converters also read and write, is what runs out first.
+// The maximum is that of the first block a row sees keys in; a later block is taken
+// against it as it is, and only when 16 of its weights sum to more than 2^14 (fp16
+// holds 65504, and keeps its 11 bits up to there) is its own maximum looked for,
+// the block redone and O rescaled in TMEM.  Blocks that no row of the CTA sees are
+// not visited, and only blocks on an edge of a row's range mask keys.
 #include "attention_kv.cuh"
 
 namespace h3b {
@@ -32,7 +32,6 @@ constexpr int kKtKeys = 128;                 // keys per block
 constexpr int kKtConvWarps = 3;
 constexpr int kKtThreads = 32 * (kKtConvWarps + 1 + 8);   // three warps a scheduler: 168 registers a thread
 constexpr int kKtUnit = 64;                  // keys a converter warp takes at a time
-constexpr int kKtChunk = 64;                 // products of a row in registers at a time
 constexpr int kKtMeta = 8;                   // blocks whose scales are kept
 constexpr float kKtMostWeight = 16384.0f;    // sum of 16 weights above which their maximum moves
 
@@ -40,26 +39,13 @@ template <int D>
 struct KvTile {
   static constexpr int kSlots = D == 64 ? 6 : 3;
   static constexpr uint32_t kTile = 128 * D * 2;           // Q, K or V tile in fp16
-  static constexpr uint32_t kP = kKtRows * kKtKeys * 2;
-  static constexpr uint32_t kSmem = 2 * kTile + kSlots * kTile + 2 * kP + kKtMeta * 8 * 16 + 256 + 1024;
+  static constexpr int kStages = D == 64 ? 3 : 2;          // units of codes a converter warp has in flight
+  static constexpr uint32_t kUnit = kKtUnit * D;           // their bytes
+  static constexpr uint32_t kSmem = (2 + kSlots) * kTile + kKtConvWarps * kStages * kUnit + kKtMeta * 8 * 16 + 384 + 1024;
 };
 
 // Some of a row's products out of TMEM.  One statement with its wait, so that no
 // use of a register moves above it.
-__device__ __forceinline__ void tmem_ld_wait(uint32_t taddr, float (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
-      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31"
-      "}, [%32];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
-        "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
-        "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
-        "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
-      : "r"(taddr)
-      : "memory");
-}
 __device__ __forceinline__ void tmem_ld_wait(uint32_t taddr, float (&r)[64]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
@@ -78,6 +64,38 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t taddr, float (&r)[64]) {
         "=f"(r[48]), "=f"(r[49]), "=f"(r[50]), "=f"(r[51]), "=f"(r[52]), "=f"(r[53]), "=f"(r[54]), "=f"(r[55]),
         "=f"(r[56]), "=f"(r[57]), "=f"(r[58]), "=f"(r[59]), "=f"(r[60]), "=f"(r[61]), "=f"(r[62]), "=f"(r[63])
       : "r"(taddr)
+      : "memory");
+}
+
+// A row's 64 words into TMEM.
+__device__ __forceinline__ void tmem_st64(uint32_t taddr, const uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x64.b32 [%0], {"
+      "%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,"
+      "%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,"
+      "%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,%64"
+      "};"
+      :
+      : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
+        "r"(r[32]), "r"(r[33]), "r"(r[34]), "r"(r[35]), "r"(r[36]), "r"(r[37]), "r"(r[38]), "r"(r[39]),
+        "r"(r[40]), "r"(r[41]), "r"(r[42]), "r"(r[43]), "r"(r[44]), "r"(r[45]), "r"(r[46]), "r"(r[47]),
+        "r"(r[48]), "r"(r[49]), "r"(r[50]), "r"(r[51]), "r"(r[52]), "r"(r[53]), "r"(r[54]), "r"(r[55]),
+        "r"(r[56]), "r"(r[57]), "r"(r[58]), "r"(r[59]), "r"(r[60]), "r"(r[61]), "r"(r[62]), "r"(r[63])
+      : "memory");
+}
+
+// D[tmem] (+)= A[tmem] * B, fp16 x fp16 -> fp32; A: row in the lane, two elements a column.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
@@ -131,60 +149,47 @@ __device__ __forceinline__ float score_scale(float x_scale, float back) { return
 __device__ __noinline__ float row_max(uint32_t taddr, uint32_t meta, float back) {
   float top = -INFINITY;
 #pragma unroll 1
-  for (int u = 0; u < 8; u += 2) {
-    float x[32];
-    tmem_ld_wait(taddr + 16 * u, x);
+  for (int h = 0; h < 2; ++h) {
+    float x[64];
+    tmem_ld_wait(taddr + 64 * h, x);
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
-      float a = x[16 * v];
+    for (int u = 0; u < 4; ++u) {
+      float a = x[16 * u];
 #pragma unroll
-      for (int k = 1; k < 16; ++k) a = fmaxf(a, x[16 * v + k]);
-      const float4 f = meta_load(meta + 16 * (u + v));
+      for (int k = 1; k < 16; ++k) a = fmaxf(a, x[16 * u + k]);
+      const float4 f = meta_load(meta + 64 * h + 16 * u);
       top = fmaxf(top, __fmaf_rn(a, score_scale(f.x, back), f.y));
     }
   }
   return top;
 }
 
-// Weights of a row's products, rounded to fp16 into its row of P; returns the sum
-// of weight / vs, and in `most` a bound of the largest weight.  kKtChunk products
-// are in registers at a time: with all 128 the loop has no registers left to keep
-// the exponentials going.
-template <int D>
-__device__ __forceinline__ float weights(uint32_t taddr, uint32_t meta, float back, float ref, uint32_t prow, int row,
+// Weights of half kHalf of a row's products, rounded to fp16 pairs; returns the
+// sum of weight / vs, and keeps in `most` a bound of the largest weight.
+template <int kHalf>
+__device__ __forceinline__ float weights(uint32_t taddr, uint32_t meta, float back, float ref, uint32_t (&w)[64],
                                          float& most) {
+  float x[64];
+  tmem_ld_wait(taddr + 64 * kHalf, x);
   float sum = 0.0f;
-  most = 0.0f;
 #pragma unroll
-  for (int c = 0; c < kKtKeys / kKtChunk; ++c) {
-    float x[kKtChunk];
-    tmem_ld_wait(taddr + kKtChunk * c, x);
+  for (int u = 0; u < 4; ++u) {
+    const float4 f = meta_load(meta + 64 * kHalf + 16 * u);
+    const float sc = score_scale(f.x, back), sh = f.y - ref;
+    uint64_t acc = 0;
 #pragma unroll
-    for (int u = 0; u < kKtChunk / 16; ++u) {
-      const float4 f = meta_load(meta + kKtChunk * c + 16 * u);
-      const float sc = score_scale(f.x, back), sh = f.y - ref;
-      uint64_t acc = 0;
-#pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int k = 16 * u + 8 * v + 2 * e;
-          float x0, x1;
-          f2_unpack(f2_fma(f2_pack(x[k], x[k + 1]), f2_pack(sc, sc), f2_pack(sh, sh)), x0, x1);
-          const float w0 = ex2_approx(x0), w1 = ex2_approx(x1);
-          acc = f2_add(acc, f2_pack(w0, w1));
-          w[e] = h2_bits(__floats2half2_rn(w0, w1));
-        }
-        const int q = (kKtChunk / 8) * c + 2 * u + v;
-        st_shared_v4(prow + (q >> 3) * (KvTile<D>::kP / 2) + (((q & 7) ^ (row & 7)) << 4),
-                     make_uint4(w[0], w[1], w[2], w[3]));
-      }
-      float a0, a1;
-      f2_unpack(acc, a0, a1);
-      most = fmaxf(most, a0 + a1);
-      sum = __fmaf_rn(a0 + a1, f.z, sum);
+    for (int e = 0; e < 8; ++e) {
+      const int k = 16 * u + 2 * e;
+      float x0, x1;
+      f2_unpack(f2_fma(f2_pack(x[k], x[k + 1]), f2_pack(sc, sc), f2_pack(sh, sh)), x0, x1);
+      const float w0 = ex2_approx(x0), w1 = ex2_approx(x1);
+      acc = f2_add(acc, f2_pack(w0, w1));
+      w[32 * kHalf + 8 * u + e] = h2_bits(__floats2half2_rn(w0, w1));
     }
+    float a0, a1;
+    f2_unpack(acc, a0, a1);
+    most = fmaxf(most, a0 + a1);
+    sum = __fmaf_rn(a0 + a1, f.z, sum);
   }
   return sum;
 }
@@ -197,18 +202,18 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sq = smem;
   uint8_t* ring = sq + 2 * L::kTile;
-  uint8_t* sp = ring + NS * L::kTile;
-  float4* s_meta = reinterpret_cast<float4*>(sp + 2 * L::kP);      // [block % 8][16 keys]: x scale, log2 vs, 1/vs
+  uint8_t* staged = ring + NS * L::kTile;                          // [converter warp][stage]
+  float4* s_meta = reinterpret_cast<float4*>(staged + kKtConvWarps * L::kStages * L::kUnit);      // [block % 8][16 keys]: x scale, log2 vs, 1/vs
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_meta + kKtMeta * 8);
   uint64_t* q_full = bars;
   uint64_t* slot_full = bars + 1;
   uint64_t* slot_empty = slot_full + NS;
   uint64_t* s_full = slot_empty + NS;      // [tile]
-  uint64_t* s_empty = s_full + 2;
-  uint64_t* p_full = s_empty + 2;
+  uint64_t* p_full = s_full + 2;
   uint64_t* o_full = p_full + 2;
   uint64_t* meta_full = o_full + 2;        // [kKtMeta]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(meta_full + kKtMeta);
+  uint64_t* staged_full = meta_full + kKtMeta;                     // [converter warp][stage]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(staged_full + kKtConvWarps * L::kStages);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -245,11 +250,11 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&s_empty[t], 128);
       mbar_init(&p_full[t], 128);
       mbar_init(&o_full[t], 1);
     }
     for (int s = 0; s < kKtMeta; ++s) mbar_init(&meta_full[s], kKtKeys / kKtUnit);
+    for (int s = 0; s < kKtConvWarps * L::kStages; ++s) mbar_init(&staged_full[s], 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -262,68 +267,85 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // ring position of K_j and V_j: K0 K1 V0 K2 V1 ...
-  auto seq_k = [](int j) { return j == 0 ? 0 : 2 * j - 1; };
-  auto seq_v = [n_blocks](int j) { return min(2 * j + 2, 2 * n_blocks - 1); };
-
   if (warp < kKtConvWarps) {
     // ----------------------------- codes to fp16 -----------------------------
     // The warps take half tiles (64 keys) in turn: unit g is half g & 1 of the
-    // tile with ring position g >> 1.  A lane's vectors of 16 codes lie 32 lanes
-    // apart, so that vector i's keys are all in 16-key group i * 4 / kVecs of the
-    // unit, whose place lane i * 4 / kVecs looked up.
-    constexpr int kPerKey = D / 16;                        // vectors of a key
-    constexpr int kVecs = kKtUnit * kPerKey / 32;
+    // tile with ring position g >> 1 (even: K, odd: V, of block g >> 2).  A unit's
+    // codes come by bulk copies (a page's codes of one head are contiguous) into
+    // one of the warp's stages, kStages units ahead.  What no page holds is
+    // converted as it lies there: codes are finite, and those keys weigh nothing.
+    constexpr int kPerKey = D / 16;                        // vectors of 16 codes of a key
+    constexpr int kVecs = kKtUnit * kPerKey / 32;          // of a unit, a lane
     constexpr int kKeyStep = 32 / kPerKey;
     const int key_in = lane / kPerKey, col = lane % kPerKey;
     const int units = 4 * n_blocks;
-    auto tile_of = [n_blocks](int seq, bool& is_v) {   // the block whose K or V has ring position seq
-      const bool end = seq == 2 * n_blocks - 1;
-      is_v = end || (seq > 0 && !(seq & 1));
-      return end ? n_blocks - 1 : is_v ? seq / 2 - 1 : (seq + 1) / 2;
+    const int seg_keys = min(p.c.page, kKtUnit), segs = kKtUnit / seg_keys;
+    const uint32_t seg_bytes = seg_keys * D;
+    const uint32_t stage0 = smem_u32(staged + warp * L::kStages * L::kUnit);
+    uint64_t* full = staged_full + warp * L::kStages;
+    auto unit_key = [&](int g) { return (blk0 + (g >> 2)) * kKtKeys + (g & 1) * kKtUnit; };
+    auto fetch_page = [&](int g, int in) {   // the page of the key `in` places into unit g
+      const int key = unit_key(g) + in;
+      return g < units && in < kKtUnit && key < len ? kv_page(p.c, b, key >> p.c.page_shift) : -1;
     };
-    // loads run ahead of their use: page numbers two of the warp's units, codes and scales one
-    auto fetch_page = [&](int g) {       // lanes 0..3: the page of their 16 keys
-      int page = -1;
-      if (lane < 4 && g < units) {
-        bool is_v;
-        const int key = (blk0 + tile_of(g >> 1, is_v)) * kKtKeys + (g & 1) * kKtUnit + 16 * lane;
-        if (key < len) page = kv_page(p.c, b, key >> p.c.page_shift);
+    auto issue = [&](int g, int stage, int page) {   // lane j copies segment j
+      const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+      if (lane == 0) mbar_arrive_expect_tx(&full[stage], seg_bytes * __popc(there));
+      __syncwarp();
+      if (page >= 0) {
+        const int key = unit_key(g) + lane * seg_keys;
+        const int64_t off = ((static_cast<int64_t>(page) * p.c.heads + hk) * p.c.page + (key & (p.c.page - 1))) * D;
+        bulk_load(stage0 + stage * L::kUnit + lane * seg_bytes, p.c.code[(g >> 1) & 1] + off, seg_bytes,
+                  smem_u32(&full[stage]));
       }
-      return page;
     };
-    uint4 codes[kVecs];
+    auto next_k = [&](int g) {     // the warp's first K unit after g
+      do g += kKtConvWarps;
+      while (g < units && ((g >> 1) & 1));
+      return g;
+    };
+    // scales of a K unit's four groups of 16 keys, in lanes 0..3: asked for one K unit ahead, their page
+    // numbers two (a number is looked at only when it is needed, so that no load is waited for)
     float ks = 0.0f, vs = 0.0f;
-    bool have = false;                   // lanes 0..3: their keys have a page
-    auto fetch = [&](int g, int page) {  // zeros where no page holds the key
-      bool is_v;
-      const int key = (blk0 + tile_of(g >> 1, is_v)) * kKtKeys + (g & 1) * kKtUnit + 16 * lane;
-      const int64_t ph = static_cast<int64_t>(page) * p.c.heads + hk;
-      have = page >= 0;
-      int64_t off = -1;
+    bool have = false;
+    int slot_k = -1, page_k = -1;
+    auto ask_page = [&](int g) {
+      const int key = unit_key(g) + 16 * lane;
+      slot_k = lane < 4 && g < units && key < len ? key >> p.c.page_shift : -1;
+      page_k = -1;
+      if (static_cast<unsigned>(slot_k) < static_cast<unsigned>(p.c.width))
+        page_k = p.c.table[static_cast<int64_t>(b) * p.c.width + slot_k];
+    };
+    auto ask_scales = [&]() {
+      have = static_cast<unsigned>(page_k) < static_cast<unsigned>(p.c.num_pages);
       if (have) {
-        off = (ph * p.c.page + (key & (p.c.page - 1))) * D;
-        if (!is_v) {
-          ks = p.c.scale[0][ph];
-          vs = p.c.scale[1][ph];
-        }
-      }
-      const int8_t* base = p.c.code[is_v] + key_in * D + 16 * col;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const int64_t at = __shfl_sync(0xffffffffu, off, w);
-#pragma unroll
-        for (int i = 0; i < kVecs / 4; ++i)
-          codes[w * (kVecs / 4) + i] =
-              at >= 0 ? __ldg(reinterpret_cast<const uint4*>(base + at + i * kKeyStep * D)) : make_uint4(0u, 0u, 0u, 0u);
+        const int64_t ph = static_cast<int64_t>(page_k) * p.c.heads + hk;
+        ks = p.c.scale[0][ph];
+        vs = p.c.scale[1][ph];
       }
     };
-    int page = fetch_page(warp);
-    if (warp < units) fetch(warp, page);
-    page = fetch_page(warp + kKtConvWarps);
-    for (int g = warp; g < units; g += kKtConvWarps) {
-      bool is_v;
-      const int seq = g >> 1, j = tile_of(seq, is_v), s = seq % NS;
+    auto seg_page = [&](int g) { return fetch_page(g, lane < segs ? lane * seg_keys : kKtUnit); };
+#pragma unroll
+    for (int st = 0; st < L::kStages; ++st)
+      if (warp + st * kKtConvWarps < units) issue(warp + st * kKtConvWarps, st, seg_page(warp + st * kKtConvWarps));
+    const int first_k = (warp >> 1) & 1 ? next_k(warp) : warp;
+    ask_page(first_k);
+    ask_scales();
+    ask_page(next_k(first_k));
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    int g = warp;
+    for (; g < units; g += kKtConvWarps) {
+      const bool is_v = (g >> 1) & 1;
+      const int seq = g >> 1, j = g >> 2, s = seq % NS;
+      // the page of the unit that takes this stage next: asked for now, used at the end
+      const int after = g + L::kStages * kKtConvWarps;
+      const int key_after = unit_key(after) + lane * seg_keys;
+      int slot_after = -1, page_after = -1;
+      if (after < units && lane < segs && key_after < len) slot_after = key_after >> p.c.page_shift;
+      if (static_cast<unsigned>(slot_after) < static_cast<unsigned>(p.c.width))
+        page_after = p.c.table[static_cast<int64_t>(b) * p.c.width + slot_after];
       // A page with a NaN scale gets NaN keys instead, so that it reaches the rows that see it and no other.
       unsigned poisoned = 0;
       if (!is_v) {
@@ -338,8 +360,12 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&meta_full[j % kKtMeta]);
+        ask_scales();
+        ask_page(next_k(next_k(g)));
       }
-      if (!__all_sync(0xffffffffu, mbar_wait(&slot_empty[s], ((seq / NS) & 1) ^ 1, abort_flag))) break;
+      ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, abort_flag) &&
+                                       mbar_wait(&slot_empty[s], ((seq / NS) & 1) ^ 1, abort_flag));
+      if (!ok) break;
       // 16-byte chunks 2 (col % 4) and + 1 of the key's 128-byte row; the second half of the head's dims
       // writes them in the other order, which keeps the eight lanes of a store in different banks
       const int swap = col >> 2;
@@ -351,21 +377,28 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
         at0[i] = dst + (((2 * (col & 3) + swap) ^ r) << 4);
         at1[i] = dst + (((2 * (col & 3) + 1 - swap) ^ r) << 4);
       }
+      const uint4* src = reinterpret_cast<const uint4*>(staged + (warp * L::kStages + stage) * L::kUnit) + lane;
 #pragma unroll
-      for (int i = 0; i < kVecs; ++i) {
-        const uint32_t w[4] = {codes[i].x ^ 0x80808080u, codes[i].y ^ 0x80808080u, codes[i].z ^ 0x80808080u,
-                               codes[i].w ^ 0x80808080u};
-        uint32_t h[8];
+      for (int i0 = 0; i0 < kVecs; i0 += 8) {
+        uint4 codes[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          h[2 * e] = codes_to_h2(w[e], 0x4140);
-          h[2 * e + 1] = codes_to_h2(w[e], 0x4342);
+        for (int i = 0; i < 8; ++i) codes[i] = src[32 * (i0 + i)];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t w[4] = {codes[i].x ^ 0x80808080u, codes[i].y ^ 0x80808080u, codes[i].z ^ 0x80808080u,
+                                 codes[i].w ^ 0x80808080u};
+          uint32_t h[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            h[2 * e] = codes_to_h2(w[e], 0x4140);
+            h[2 * e + 1] = codes_to_h2(w[e], 0x4342);
+          }
+          const int v = kVecs > 8 ? i & 1 : 0;
+          st_shared_v4(at0[v] + (i0 + i) * kKeyStep * 128,
+                       swap ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(h[0], h[1], h[2], h[3]));
+          st_shared_v4(at1[v] + (i0 + i) * kKeyStep * 128,
+                       swap ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(h[4], h[5], h[6], h[7]));
         }
-        const int v = kVecs > 8 ? i & 1 : 0;
-        st_shared_v4(at0[v] + i * kKeyStep * 128,
-                     swap ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(h[0], h[1], h[2], h[3]));
-        st_shared_v4(at1[v] + i * kKeyStep * 128,
-                     swap ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(h[4], h[5], h[6], h[7]));
       }
       if (poisoned) {
         const uint4 nan = make_uint4(0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u);
@@ -380,8 +413,20 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&slot_full[s]);
-      if (g + kKtConvWarps < units) fetch(g + kKtConvWarps, page);
-      page = fetch_page(g + 2 * kKtConvWarps);
+      if (after < units) {
+        if (slot_after >= 0 && static_cast<unsigned>(page_after) >= static_cast<unsigned>(p.c.num_pages)) {
+          record_error(kErrKvPage);
+          page_after = -1;
+        }
+        issue(after, stage, page_after);
+      }
+      if (++stage == L::kStages) stage = 0, phase ^= 1;
+    }
+    if (!ok) {   // let the copies in flight land before the block's memory goes
+      for (int st = 1; st < L::kStages; ++st) {
+        if (++stage == L::kStages) stage = 0, phase ^= 1;
+        if (g + st * kKtConvWarps < units) mbar_wait(&full[stage], phase, nullptr);
+      }
     }
   } else if (warp == 3) {
     // ------------------------------- MMA issuer -------------------------------
@@ -390,9 +435,8 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
       constexpr uint32_t idesc_pv = make_idesc_f16(kKtRows, D) | (1u << 16);   // V is MN-major
       bool ok = n_blocks == 0 || mbar_poll(q_full, 0, abort_flag);
       auto issue_s = [&](int j, int t) -> bool {
-        const int seq = seq_k(j), s = seq % NS;
-        if (!mbar_poll(&slot_full[s], (seq / NS) & 1, abort_flag)) return false;
-        if (!mbar_poll(&s_empty[t], (j & 1) ^ 1, abort_flag)) return false;
+        const int seq = 2 * j, s = seq % NS;
+        if (t == 0 && !mbar_poll(&slot_full[s], (seq / NS) & 1, abort_flag)) return false;
         tc_fence_after();
         const uint32_t qb = smem_u32(sq + t * L::kTile), kb = smem_u32(ring + s * L::kTile);
 #pragma unroll
@@ -405,25 +449,24 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
       };
       for (int t = 0; t < tiles && ok && n_blocks > 0; ++t) ok = issue_s(0, t);
       for (int j = 0; j < n_blocks && ok; ++j) {
-        const int seq = seq_v(j), s = seq % NS;
+        const int seq = 2 * j + 1, s = seq % NS;
+        if (!mbar_poll(&slot_full[s], (seq / NS) & 1, abort_flag)) break;
         for (int t = 0; t < tiles && ok; ++t) {
-          // the softmax of block j has left S(t): the next products first, they are waited for sooner
-          if (j + 1 < n_blocks && !issue_s(j + 1, t)) { ok = false; break; }
-          if (t == 0 && !mbar_poll(&slot_full[s], (seq / NS) & 1, abort_flag)) { ok = false; break; }
           if (!mbar_poll(&p_full[t], j & 1, abort_flag)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t pb = smem_u32(sp + t * L::kP), vb = smem_u32(ring + s * L::kTile);
+          const uint32_t vb = smem_u32(ring + s * L::kTile);
 #pragma unroll
           for (int k = 0; k < kKtKeys / 16; ++k) {
             // 64 dims of 16 keys are one swizzle atom column; the next 64 dims lie 16 KB further
             uint64_t vd = make_sw128_desc(vb + k * 16 * 128);
             vd = (vd & ~(uint64_t(0x3FFFu) << 16)) | (uint64_t(16384 >> 4) << 16);
-            mma_f16(tmem + t * 256 + 128, make_sw128_desc(pb + (k >> 2) * (L::kP / 2)) + 2 * (k & 3), vd, idesc_pv,
-                    (j > 0 || k > 0) ? 1u : 0u);
+            mma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, vd, idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
           }
-          tc_commit(&o_full[t]);
+          if (j + 1 == n_blocks) tc_commit(&o_full[t]);
+          if (t == tiles - 1) tc_commit(&slot_empty[s]);
+          // The next products go where the weights were: the tensor core takes its instructions in order.
+          if (j + 1 < n_blocks) ok = issue_s(j + 1, t);
         }
-        if (ok) tc_commit(&slot_empty[s]);
       }
     }
   } else {
@@ -468,23 +511,21 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
       }
       float m = -INFINITY, l = 0.0f;
       bool ok = true;
-      const uint32_t prow = smem_u32(sp + tile * L::kP + row * 128);
-      const uint32_t bar_s_full = smem_u32(&s_full[tile]), bar_s_empty = smem_u32(&s_empty[tile]);
-      const uint32_t bar_p_full = smem_u32(&p_full[tile]), bar_o_full = smem_u32(&o_full[tile]);
       for (int j = 0; j < n_blocks; ++j) {
         ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(smem_u32(&meta_full[j % kKtMeta]), (j / kKtMeta) & 1, abort_flag));
-        ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(bar_s_full, j & 1, abort_flag));
+        // S(j) is there, and with it everything issued before: O holds W V up to block j - 1
+        ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(smem_u32(&s_full[tile]), j & 1, abort_flag));
         uint32_t meta = smem_u32(s_meta + (j % kKtMeta) * 8);
         asm volatile("" : "+r"(meta));     // its loads stay below the wait
         // (after a wait that gave up the values mean nothing, but every warp keeps in step)
         tc_fence_after();
         const int key0 = (blk0 + j) * kKtKeys;
         if (key0 < first_max || key0 + kKtKeys > last_min) mask_products(t_s, first - key0, last - key0);
-        if (j > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(bar_o_full, (j - 1) & 1, abort_flag));
         // Against the maximum so far; only a row without one, or whose weights outgrow fp16's range by
         // their sums, looks for this block's.
         bool look = __any_sync(0xffffffffu, m == -INFINITY), moved = false;
         float alpha = 1.0f, sum;
+        uint32_t w[64];
         while (true) {
           if (look) {
             const float m_new = fmaxf(m, row_max(t_s, meta, back));
@@ -492,25 +533,21 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
             alpha = moved ? ex2_approx(m - m_new) : 1.0f;
             m = m_new;
           }
-          float most;
-          sum = weights<D>(t_s, meta, back, m == -INFINITY ? 0.0f : m, prow, row, most);
+          const float ref = m == -INFINITY ? 0.0f : m;
+          float most = 0.0f;
+          sum = weights<0>(t_s, meta, back, ref, w, most);
+          sum += weights<1>(t_s, meta, back, ref, w, most);
           if (look || !__any_sync(0xffffffffu, most > kKtMostWeight)) break;
           look = true;
         }
-        tc_fence_before();
-        mbar_arrive_u32(bar_s_empty);
+        tmem_st64(t_s, w);      // over the products that they came from
         l = __fmaf_rn(l, alpha, sum);
-        if (ok && j > 0) {
-          tc_fence_after();
-          if (__any_sync(0xffffffffu, moved)) rescale_row(t_o, D, alpha);
-        }
-        if (ok) {
-          tc_fence_before();
-          fence_proxy_async_smem();
-          mbar_arrive_u32(bar_p_full);
-        }
+        if (j > 0 && __any_sync(0xffffffffu, moved)) rescale_row(t_o, D, alpha);
+        tmem_st_wait();
+        tc_fence_before();
+        if (ok) mbar_arrive(&p_full[tile]);
       }
-      if (n_blocks > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(bar_o_full, (n_blocks - 1) & 1, abort_flag));
+      if (n_blocks > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(smem_u32(&o_full[tile]), 0, abort_flag));
       const bool have = ok && n_blocks > 0;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       if (have) tc_fence_after();
