@@ -304,34 +304,40 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
       while (g < units && ((g >> 1) & 1));
       return g;
     };
-    // scales of a K unit's four groups of 16 keys, in lanes 0..3: asked for one K unit ahead, their page
-    // numbers two (a number is looked at only when it is needed, so that no load is waited for)
-    float ks = 0.0f, vs = 0.0f;
-    bool have = false;
-    int slot_k = -1, page_k = -1;
-    auto ask_page = [&](int g) {
-      const int key = unit_key(g) + 16 * lane;
-      slot_k = lane < 4 && g < units && key < len ? key >> p.c.page_shift : -1;
-      page_k = -1;
-      if (static_cast<unsigned>(slot_k) < static_cast<unsigned>(p.c.width))
-        page_k = p.c.table[static_cast<int64_t>(b) * p.c.width + slot_k];
+    // Global loads are asked for ahead and not looked at before they are needed, so that none is waited for:
+    // the page numbers of a unit's copies one unit before the copies, a K unit's scales two K units before
+    // their use (lanes 0..3: its four groups of 16 keys) and their page numbers three.
+    auto ask_page = [&](int key, bool want) {
+      const int slot = key >> p.c.page_shift;
+      return want && key < len && static_cast<unsigned>(slot) < static_cast<unsigned>(p.c.width)
+                 ? p.c.table[static_cast<int64_t>(b) * p.c.width + slot] : -1;
     };
-    auto ask_scales = [&]() {
-      have = static_cast<unsigned>(page_k) < static_cast<unsigned>(p.c.num_pages);
-      if (have) {
-        const int64_t ph = static_cast<int64_t>(page_k) * p.c.heads + hk;
-        ks = p.c.scale[0][ph];
-        vs = p.c.scale[1][ph];
+    struct Scales {
+      float k, v;
+      bool have;
+    };
+    auto ask_k_page = [&](int g) { return ask_page(unit_key(g) + 16 * lane, lane < 4 && g < units); };
+    auto ask_scales = [&](int page) {
+      Scales r{0.0f, 0.0f, static_cast<unsigned>(page) < static_cast<unsigned>(p.c.num_pages)};
+      if (r.have) {
+        const int64_t ph = static_cast<int64_t>(page) * p.c.heads + hk;
+        r.k = p.c.scale[0][ph];
+        r.v = p.c.scale[1][ph];
       }
+      return r;
     };
     auto seg_page = [&](int g) { return fetch_page(g, lane < segs ? lane * seg_keys : kKtUnit); };
 #pragma unroll
     for (int st = 0; st < L::kStages; ++st)
       if (warp + st * kKtConvWarps < units) issue(warp + st * kKtConvWarps, st, seg_page(warp + st * kKtConvWarps));
-    const int first_k = (warp >> 1) & 1 ? next_k(warp) : warp;
-    ask_page(first_k);
-    ask_scales();
-    ask_page(next_k(first_k));
+    int k2 = (warp >> 1) & 1 ? next_k(warp) : warp;         // the K unit whose page is asked for last
+    Scales now = ask_scales(ask_k_page(k2));
+    k2 = next_k(k2);
+    Scales then = ask_scales(ask_k_page(k2));
+    k2 = next_k(k2);
+    int page_k = ask_k_page(k2);
+    int page_next = ask_page(unit_key(warp + L::kStages * kKtConvWarps) + lane * seg_keys,
+                             lane < segs && warp + L::kStages * kKtConvWarps < units);
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -339,29 +345,25 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
     for (; g < units; g += kKtConvWarps) {
       const bool is_v = (g >> 1) & 1;
       const int seq = g >> 1, j = g >> 2, s = seq % NS;
-      // the page of the unit that takes this stage next: asked for now, used at the end
-      const int after = g + L::kStages * kKtConvWarps;
-      const int key_after = unit_key(after) + lane * seg_keys;
-      int slot_after = -1, page_after = -1;
-      if (after < units && lane < segs && key_after < len) slot_after = key_after >> p.c.page_shift;
-      if (static_cast<unsigned>(slot_after) < static_cast<unsigned>(p.c.width))
-        page_after = p.c.table[static_cast<int64_t>(b) * p.c.width + slot_after];
+      const int after = g + L::kStages * kKtConvWarps;     // the unit that takes this stage next
       // A page with a NaN scale gets NaN keys instead, so that it reaches the rows that see it and no other.
       unsigned poisoned = 0;
       if (!is_v) {
-        poisoned = __ballot_sync(0xffffffffu, have && (isnan(ks) || isnan(vs)));
+        poisoned = __ballot_sync(0xffffffffu, now.have && (isnan(now.k) || isnan(now.v)));
         if (lane < 4) {
           float4 f = make_float4(1.0f, -INFINITY, 0.0f, 0.0f);       // no page: weight 0
-          if (have) {   // a scale of zero: a page never written holds zeros
-            const float v = fmaxf(vs, kKvMinScale);
-            f = make_float4(fmaxf(ks, kKvMinScale) * fabsf(p.scale_log2), log2f(v), __frcp_rn(v), 0.0f);
+          if (now.have) {   // a scale of zero: a page never written holds zeros
+            const float v = fmaxf(now.v, kKvMinScale);
+            f = make_float4(fmaxf(now.k, kKvMinScale) * fabsf(p.scale_log2), log2f(v), __frcp_rn(v), 0.0f);
           }
           s_meta[(j % kKtMeta) * 8 + (g & 1) * 4 + lane] = f;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&meta_full[j % kKtMeta]);
-        ask_scales();
-        ask_page(next_k(next_k(g)));
+        now = then;
+        then = ask_scales(page_k);
+        k2 = next_k(k2);
+        page_k = ask_k_page(k2);
       }
       ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, abort_flag) &&
                                        mbar_wait(&slot_empty[s], ((seq / NS) & 1) ^ 1, abort_flag));
@@ -414,11 +416,13 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
       __syncwarp();
       if (lane == 0) mbar_arrive(&slot_full[s]);
       if (after < units) {
-        if (slot_after >= 0 && static_cast<unsigned>(page_after) >= static_cast<unsigned>(p.c.num_pages)) {
-          record_error(kErrKvPage);
-          page_after = -1;
+        if (static_cast<unsigned>(page_next) >= static_cast<unsigned>(p.c.num_pages)) {
+          if (lane < segs && unit_key(after) + lane * seg_keys < len) record_error(kErrKvPage);
+          page_next = -1;
         }
-        issue(after, stage, page_after);
+        issue(after, stage, page_next);
+        page_next = ask_page(unit_key(after + kKtConvWarps) + lane * seg_keys,
+                             lane < segs && after + kKtConvWarps < units);
       }
       if (++stage == L::kStages) stage = 0, phase ^= 1;
     }

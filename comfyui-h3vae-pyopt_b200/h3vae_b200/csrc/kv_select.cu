@@ -20,10 +20,10 @@ struct KvSelectParams {
   const void* q;
   const int32_t* lengths;
   const int32_t* counts;
-  uint32_t* keys;        // [batch, heads, tokens, width]
+  uint32_t* keys;        // [batch, heads, tokens, row_keys]
   int32_t* selected;
   int64_t qs[3];
-  int group, tokens, n;
+  int group, tokens, n, row_keys;
 };
 
 // Last page ordinal row t of sequence b sees, -1 if none.
@@ -87,47 +87,53 @@ __global__ void __launch_bounds__(kSelThreads) kv_score_kernel(const KvSelectPar
       __syncthreads();
       if (page >= 0) {
         for (int r = 0; r < rows; ++r) {
-          int dot = 0;
+          int dots[4] = {0, 0, 0, 0};       // four chains, so that they run into one another's latency
 #pragma unroll
-          for (int i = 0; i < D / 4; ++i) {
-            const int w = static_cast<int>(s_q[r][i]);
-            dot = __dp2a_lo(static_cast<int>(k[2 * i]), w, dot);
-            dot = __dp2a_hi(static_cast<int>(k[2 * i + 1]), w, dot);
+          for (int i = 0; i < D / 4; i += 4) {
+            const uint4 q4 = *reinterpret_cast<const uint4*>(&s_q[r][i]);
+            const uint32_t w[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              dots[e] = __dp2a_lo(static_cast<int>(k[2 * (i + e)]), static_cast<int>(w[e]), dots[e]);
+              dots[e] = __dp2a_hi(static_cast<int>(k[2 * (i + e) + 1]), static_cast<int>(w[e]), dots[e]);
+            }
           }
-          const float x = __fmul_rn(static_cast<float>(dot), s_s[r]);
+          const float x = __fmul_rn(static_cast<float>((dots[0] + dots[1]) + (dots[2] + dots[3])), s_s[r]);
           const int g = r % gn;
           best = g0 + g == 0 ? x : fmaxf(best, x);
           if (g0 + g + 1 == p.group) {
             const float y = __fadd_rn(__fmul_rn(best, k_scale), 0.0f);   // -0 becomes +0
             const uint32_t key = isnan(y) ? 0xffffffffu : float_to_ordered(y);
             const int64_t row = (static_cast<int64_t>(b) * p.c.heads + head) * p.tokens + t0 + r / gn;
-            p.keys[row * p.c.width + slot] = key;
+            p.keys[row * p.row_keys + slot] = key;
           }
         }
       } else if (slot < last && g1 == p.group) {   // a bad page number: never worth choosing
         for (int t = t0; t < t1; ++t)
-          p.keys[((static_cast<int64_t>(b) * p.c.heads + head) * p.tokens + t) * p.c.width + slot] = 0u;
+          p.keys[((static_cast<int64_t>(b) * p.c.heads + head) * p.tokens + t) * p.row_keys + slot] = 0u;
       }
     }
   }
 }
 
 // The n - 1 best of a row's `last` keys, by bisection on the key's bits: the
-// threshold is built from the top bit down, counting the keys at or above it,
-// and found as soon as that count is right.  Each thread holds kPer consecutive
+// threshold is built from the top down, two bits a round, counting the keys at or
+// above it, and found as soon as that count is right.  Each thread holds kPer consecutive
 // keys in registers; more pages than the block holds are read again each round.
-// (A histogram of 8-bit digits met 2047 keys in a few bins and took 22 us a row;
-// this takes 2 to 3.)
-constexpr int kPickThreads = 256;
+// Four warps a row: a round is 3 kPer comparisons and one barrier, and the
+// barrier's latency is what a wider block pays for (2048 pages: 10 us with 16
+// warps, 22 us with a histogram of 8-bit digits that most keys share).
+constexpr int kPickThreads = 128;
 
 template <int kPer>
 __global__ void __launch_bounds__(kPickThreads) kv_pick_kernel(const KvSelectParams p) {
   constexpr int kWarps = kPickThreads / 32;
-  __shared__ int s_count[2][kWarps];
+  static_assert(kWarps == 4, "a round's counts are read as one vector");
+  __shared__ __align__(16) int s_count[2][3][kWarps];
   const int t = blockIdx.x, head = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t row = (static_cast<int64_t>(b) * p.c.heads + head) * p.tokens + t;
   int32_t* out = p.selected + row * p.n;
-  const uint32_t* keys = p.keys + row * p.c.width;
+  const uint32_t* keys = p.keys + row * p.row_keys;
   const int last = kv_last_page(p, b, t);
   asm volatile("griddepcontrol.wait;" ::: "memory");   // the scores; every block waits, so that none outlive this call
   if (last < p.n) {   // every page fits
@@ -142,30 +148,46 @@ __global__ void __launch_bounds__(kPickThreads) kv_pick_kernel(const KvSelectPar
   auto load = [&](int round) {
     const int i0 = (round * kPickThreads + tid) * kPer;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) k[e] = i0 + e < last ? __ldcg(keys + i0 + e) : 0u;
+    for (int e = 0; e < kPer; e += 4) {   // rows are 16-byte aligned and whole vectors long
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (i0 + e < last) v = __ldcg(reinterpret_cast<const uint4*>(keys + i0 + e));
+      k[e] = v.x;
+      k[e + 1] = i0 + e + 1 < last ? v.y : 0u;
+      k[e + 2] = i0 + e + 2 < last ? v.z : 0u;
+      k[e + 3] = i0 + e + 3 < last ? v.w : 0u;
+    }
   };
   if (rounds == 1) load(0);
-  // largest threshold with at least `want` keys at or above it (keys are never 0 but on bad pages)
+  // largest threshold with at least `want` keys at or above it, two bits a round (keys are never 0 but on bad pages)
   uint32_t thr = 0;
   int at_least = last;
-  for (int bit = 31; bit >= 0 && at_least != want; --bit) {
-    const uint32_t cand = thr | (1u << bit);
-    int n = 0;
+  for (int bit = 30; bit >= 0 && at_least != want; bit -= 2) {
+    int n[3] = {0, 0, 0};
     for (int r = 0; r < rounds; ++r) {
       if (rounds > 1) load(r);
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) n += k[e] >= cand ? 1 : 0;
-    }
-    n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) s_count[bit & 1][warp] = n;
-    __syncthreads();
-    n = 0;
+      for (int e = 0; e < kPer; ++e)
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) n += s_count[bit & 1][w];
-    if (n >= want) {
-      thr = cand;
-      at_least = n;
+        for (int c = 0; c < 3; ++c) n[c] += k[e] >= (thr | static_cast<uint32_t>(c + 1) << bit) ? 1 : 0;
     }
+    const int buf = (bit >> 1) & 1;
+#pragma unroll
+    for (int c = 0; c < 3; ++c) {
+      n[c] = __reduce_add_sync(0xffffffffu, n[c]);
+      if (lane == 0) s_count[buf][c][warp] = n[c];
+    }
+    __syncthreads();
+    int take = 0;
+#pragma unroll
+    for (int c = 0; c < 3; ++c) {
+      const int4 v = *reinterpret_cast<const int4*>(s_count[buf][c]);
+      n[c] = (v.x + v.y) + (v.z + v.w);
+      if (n[c] >= want) {
+        take = c + 1;
+        at_least = n[c];
+      }
+    }
+    thr |= static_cast<uint32_t>(take) << bit;
   }
   // keys above the threshold, and of those that equal it the first in page order
   int above = 0;
@@ -177,11 +199,11 @@ __global__ void __launch_bounds__(kPickThreads) kv_pick_kernel(const KvSelectPar
     }
     above = __reduce_add_sync(0xffffffffu, above);
     __syncthreads();
-    if (lane == 0) s_count[0][warp] = above;
+    if (lane == 0) s_count[0][0][warp] = above;
     __syncthreads();
     above = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) above += s_count[0][w];
+    for (int w = 0; w < kWarps; ++w) above += s_count[0][0][w];
   }
   const int ties = at_least != want ? want - above : last;    // that are taken
   int n_out = 0, n_tie = 0;
@@ -199,13 +221,13 @@ __global__ void __launch_bounds__(kPickThreads) kv_pick_kernel(const KvSelectPar
       if (lane >= o) incl += up;
     }
     __syncthreads();
-    if (lane == 31) s_count[1][warp] = incl;
+    if (lane == 31) s_count[1][0][warp] = incl;
     __syncthreads();
     int before = incl - mine, all = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      before += w < warp ? s_count[1][w] : 0;
-      all += s_count[1][w];
+      before += w < warp ? s_count[1][0][w] : 0;
+      all += s_count[1][0][w];
     }
     int tie = n_tie + (before & 0xffff);
     int at = n_out + (before >> 16) + min(tie, ties) - min(n_tie, ties);
@@ -226,7 +248,7 @@ __global__ void __launch_bounds__(kPickThreads) kv_pick_kernel(const KvSelectPar
 extern "C" size_t h3b_kv_select_i8_workspace_size(int64_t batch, int64_t kv_heads, int64_t tokens,
                                                   int64_t table_width) {
   if (batch <= 0 || kv_heads <= 0 || tokens <= 0 || table_width <= 0) return 16;
-  return ((size_t)batch * kv_heads * tokens * table_width * 4 + 15) & ~size_t(15);
+  return (size_t)batch * kv_heads * tokens * ((table_width + 3) & ~int64_t(3)) * 4;
 }
 
 extern "C" int h3b_kv_select_i8(const void* q, const int64_t* q_strides, const h3b_kv_cache* cache,
@@ -257,6 +279,7 @@ extern "C" int h3b_kv_select_i8(const void* q, const int64_t* q_strides, const h
   p.group = (int)(q_heads / cache->kv_heads);
   p.tokens = (int)tokens;
   p.n = (int)n_selected;
+  p.row_keys = (int)((table_width + 3) & ~int64_t(3));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   dim3 g1((unsigned)((table_width + h3b::kSelThreads - 1) / h3b::kSelThreads), (unsigned)cache->kv_heads, (unsigned)batch);
   dim3 g2((unsigned)tokens, (unsigned)cache->kv_heads, (unsigned)batch);
@@ -279,8 +302,10 @@ extern "C" int h3b_kv_select_i8(const void* q, const int64_t* q_strides, const h
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  cudaError_t e = table_width <= 4 * h3b::kPickThreads ? cudaLaunchKernelEx(&cfg, h3b::kv_pick_kernel<4>, p)
-                                                       : cudaLaunchKernelEx(&cfg, h3b::kv_pick_kernel<16>, p);
+  cudaError_t e = table_width <= 4 * h3b::kPickThreads    ? cudaLaunchKernelEx(&cfg, h3b::kv_pick_kernel<4>, p)
+                  : table_width <= 8 * h3b::kPickThreads  ? cudaLaunchKernelEx(&cfg, h3b::kv_pick_kernel<8>, p)
+                  : table_width <= 20 * h3b::kPickThreads ? cudaLaunchKernelEx(&cfg, h3b::kv_pick_kernel<20>, p)
+                                                          : cudaLaunchKernelEx(&cfg, h3b::kv_pick_kernel<64>, p);
   if (e != cudaSuccess) return h3b_host::set_error(H3B_ECUDA, "%s: selection launch: %s", name, cudaGetErrorString(e));
   return h3b_host::check_launch(name);
 }
