@@ -8,8 +8,15 @@
 
 namespace {
 
-// Rows of a (sequence, kv head) above which the tensor-core tiles are taken.
-constexpr int64_t kTileRows = 64;
+// The tensor-core tiles are taken above kTileRows rows of a (sequence, kv head)
+// if the 16-row tiles of the other kernel would read more than kTileBytes of
+// codes.  Measured, tiles against 16-row tiles, us: 16 heads over 5120 keys, dim 64:
+// 33 rows 19.5 / 14.7, 64 rows 19.9 / 26.4; 8 x 8 heads over 8192 keys, dim 128: 20
+// rows 78 / 77, 36 rows 79 / 99, 128 rows 83 / 225; 32 x 16 heads over 2000 keys: 40
+// rows 130 / 97, 70 rows 131 / 151; 8 heads over 1000 keys, dim 128: 128 rows (16 MB)
+// 22 / 12, 256 rows (33 MB) 28 / 28.
+constexpr int64_t kTileRows = 48;
+constexpr int64_t kTileBytes = int64_t(24) << 20;
 
 // The plan of a call.  tile: attention_kv_tile_kernel, 256 rows a block, the
 // keys in `slots` parts.  Otherwise attention_kv_split_kernel: rows in tiles of
@@ -29,7 +36,9 @@ KvPlan kv_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens,
   const int64_t keys = kSplitStageBytes / 2 / dim;
   const int64_t most = (kSplitPages - 1) * page / keys;    // tiles a run may have: it may start inside a page
   const int64_t rows = n_selected > 0 ? group : group * tokens;
-  k.tile = n_selected <= 0 && rows > kTileRows;
+  const int64_t row_tiles = (rows + kSplitRows - 1) / kSplitRows;
+  k.tile = n_selected <= 0 && rows > kTileRows &&
+           batch * kv_heads * row_tiles > kTileBytes / (2 * dim * width * page);
   if (k.tile) {
     k.row_tiles = (rows + 2 * kKtRows - 1) / (2 * kKtRows);
     const int64_t blocks = batch * kv_heads * k.row_tiles, most_blocks = (width * page + kKtKeys - 1) / kKtKeys;
@@ -37,7 +46,7 @@ KvPlan kv_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens,
     k.part_bytes = k.slots > 1 ? (size_t)(k.slots * batch * kv_heads * rows) * (dim + 4) * 4 : 0;
     return k;
   }
-  k.row_tiles = (rows + kSplitRows - 1) / kSplitRows;
+  k.row_tiles = row_tiles;
   // one wave of blocks over selected pages, two over ragged lengths (measured on 16 x 48 pages: 27, 29, 32 us for
   // one, two, three; on 16 x 6553..32768 keys: 158, 139, 139)
   k.target = (n_selected > 0 ? 1 : 2) * kSplitBlocks * h3b_host::num_sms();

@@ -23,6 +23,12 @@ def _tables(rng, lens, page, spare=3, width=None):
     return rows, _i32([r + [-1] * (width - len(r)) for r in rows]), sum(need) + spare
 
 
+def _wide(table, pages=20000):
+    """The same table in rows of many more pages: calls are planned for what a table could hold, so small lengths
+    then run on the kernels for long sequences (parts joined by a second kernel, tensor-core row tiles)."""
+    return torch.nn.functional.pad(table, (0, pages - table.shape[1]), value=-1).contiguous()
+
+
 def _rounded(x, dtype):
     """fp32 numpy of x rounded to dtype."""
     return torch.from_numpy(np.ascontiguousarray(x, np.float32)).to(TYPES[dtype]).float().numpy()
@@ -261,13 +267,15 @@ CASES = [
 ]
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("case", range(len(CASES)))
-def test_attention(cuda_lib, case):
+def test_attention(cuda_lib, case, wide):
     from h3vae_b200 import kernels as K
     dtype, dim, page, heads, group, t, lens, counts, causal, window = CASES[case]
     rng = np.random.default_rng(100 + case)
     ref, rows, table = _filled(rng, lens, heads, dim, page)
     cache = _cache(ref)
+    table = _wide(table) if wide else table
     batch = len(lens)
     q = torch.from_numpy(rng.standard_normal((batch, heads * group, t, dim)) * 2).to(TYPES[dtype]).cuda()
     args = dict(causal=causal, window=window)
@@ -286,13 +294,15 @@ def test_attention(cuda_lib, case):
 
 @pytest.mark.parametrize("t,group", [(1, 1), (1, 12), (3, 8), (150, 1), (40, 4)])
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
-def test_attention_layouts(cuda_lib, t, group, dtype):
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_layouts(cuda_lib, t, group, dtype, wide):
     """Transposed, interleaved and unaligned q and out give the bits of dense ones."""
     from h3vae_b200 import kernels as K
     rng = np.random.default_rng(5)
     lens = [310, 151]
     ref, rows, table = _filled(rng, lens, 2, 64, 64)
     cache = _cache(ref)
+    table = _wide(table) if wide else table
     q = torch.from_numpy(rng.standard_normal((2, 2 * group, t, 64))).to(TYPES[dtype]).cuda()
     want = K.attention_kv_i8(q, cache, table, _i32(lens), 0.125)
     wide = torch.zeros(2, t, 2 * group, 3 * 64 + 1, dtype=q.dtype, device="cuda")
@@ -305,19 +315,20 @@ def test_attention_layouts(cuda_lib, t, group, dtype):
 
 
 @pytest.mark.parametrize("t", [1, 9, 140])
-def test_masked_places_have_no_effect(cuda_lib, t):
+@pytest.mark.parametrize("wide", [False, True])
+def test_masked_places_have_no_effect(cuda_lib, t, wide):
     """NaN scales and any codes in pages and slots past what a row sees; a NaN page that some rows see makes
     exactly those rows NaN."""
     from h3vae_b200 import kernels as K
     rng = np.random.default_rng(6)
     lens, page = [150, 200], 16
     ref, rows, table = _filled(rng, lens, 2, 64, page)
-    clean, _, _ = ref, rows, table
     cache = _cache(ref)
-    wide = torch.cat([table, _i32([[rows[1][0]] * 3, [rows[0][0]] * 3])], 1).contiguous()   # more table than tokens
+    more = torch.cat([table, _i32([[rows[1][0]] * 3, [rows[0][0]] * 3])], 1).contiguous()   # more table than tokens
+    table, more = (_wide(table), _wide(more)) if wide else (table, more)
     q = torch.from_numpy(rng.standard_normal((2, 4, t, 64))).half().cuda()
-    out, _, bound = _attend_all(clean, rows, q, lens, [t, t], 0.125, page)
-    R.check(K.attention_kv_i8(q, cache, wide, _i32(lens), 0.125), out, bound, torch.float16)
+    out, _, bound = _attend_all(ref, rows, q, lens, [t, t], 0.125, page)
+    R.check(K.attention_kv_i8(q, cache, more, _i32(lens), 0.125), out, bound, torch.float16)
     # the last page of sequence 0 turns NaN
     last = rows[0][149 // page]
     cache.k_scale[last] = float("nan")
@@ -335,8 +346,9 @@ def test_masked_places_have_no_effect(cuda_lib, t):
 
 
 @pytest.mark.parametrize("t,group", [(1, 2), (6, 12), (130, 2)])
-@pytest.mark.parametrize("scale", [0.125, 4.0, 0.0])
-def test_attention_spread_scales(cuda_lib, t, group, scale):
+@pytest.mark.parametrize("scale", [0.125, 4.0, 0.0, -0.2])
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_spread_scales(cuda_lib, t, group, scale, wide):
     """V pages whose scales differ by 10^8, zero pages among them, and near one-hot rows."""
     from h3vae_b200 import kernels as K
     rng = np.random.default_rng(7)
@@ -349,7 +361,7 @@ def test_attention_spread_scales(cuda_lib, t, group, scale):
         ref.scale["k"][row[4]] = R.TINY
     cache = _cache(ref)
     q = torch.from_numpy(rng.standard_normal((2, group, t, 64))).half().cuda()
-    got = K.attention_kv_i8(q, cache, table, _i32(lens), scale)
+    got = K.attention_kv_i8(q, cache, _wide(table) if wide else table, _i32(lens), scale)
     out, _, bound = _attend_all(ref, rows, q, lens, [t, t], scale, page)
     R.check(got, out, bound, torch.float16)
 
@@ -360,6 +372,7 @@ def test_attention_bf16_wide_queries(cuda_lib):
     rng = np.random.default_rng(8)
     ref, rows, table = _filled(rng, [200], 1, 64, 64)
     cache = _cache(ref)
+    table = _wide(table)
     for size in (1e6, 1e-6, 1e-30):
         for t in (1, 130):
             q = torch.from_numpy(rng.standard_normal((1, 2, t, 64)) * size).to(torch.bfloat16).cuda()
@@ -391,6 +404,8 @@ def test_long_cache_offsets(cuda_lib):
         q = torch.from_numpy(rng.standard_normal((1, heads, t, dim))).half().cuda()
         a = K.attention_kv_i8(q, cache, table, _i32([n]), 0.1)
         assert torch.equal(a, K.attention_kv_i8(q, small, _i32([[0, 1, 2]]), _i32([n]), 0.1))
+        a = K.attention_kv_i8(q, cache, _wide(table), _i32([n]), 0.1)
+        assert torch.equal(a, K.attention_kv_i8(q, small, _wide(_i32([[0, 1, 2]])), _i32([n]), 0.1))
         sel = K.kv_select_i8(q, cache, table, _i32([n]), 2)
         assert torch.equal(sel, K.kv_select_i8(q, small, _i32([[0, 1, 2]]), _i32([n]), 2))
         a = K.attention_kv_i8(q, cache, table, _i32([n]), 0.1, selected=sel)
@@ -485,6 +500,7 @@ def test_side_stream_and_graph(cuda_lib):
     ref, rows, table = _filled(rng, lens, 2, 64, 64)
     cache = _cache(ref)
     n = _i32(lens)
+    table = _wide(table)
     for t in (1, 130):
         q = torch.from_numpy(rng.standard_normal((2, 4, t, 64))).half().cuda()
 
