@@ -32,8 +32,11 @@ constexpr int kKtKeys = 128;                 // keys per block
 constexpr int kKtConvWarps = 3;
 constexpr int kKtThreads = 32 * (kKtConvWarps + 1 + 8);   // three warps a scheduler: 168 registers a thread
 constexpr int kKtUnit = 64;                  // keys a converter warp takes at a time
-constexpr int kKtMeta = 8;                   // blocks whose scales are kept
+constexpr int kKtBatch = 4;                  // blocks whose pages and scales are looked up together, a lane per 16 keys
+constexpr int kKtMeta = 16;                  // blocks whose pages and scales are kept
 constexpr float kKtMostWeight = 16384.0f;    // sum of 16 weights above which their maximum moves
+
+constexpr int kPoisoned = 1 << 30;           // beside a page number (below 2^30): its scale is NaN
 
 template <int D>
 struct KvTile {
@@ -203,7 +206,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
   uint8_t* sq = smem;
   uint8_t* ring = sq + 2 * L::kTile;
   uint8_t* staged = ring + NS * L::kTile;                          // [converter warp][stage]
-  float4* s_meta = reinterpret_cast<float4*>(staged + kKtConvWarps * L::kStages * L::kUnit);      // [block % 8][16 keys]: x scale, log2 vs, 1/vs
+  float4* s_meta = reinterpret_cast<float4*>(staged + kKtConvWarps * L::kStages * L::kUnit);      // [block % 16][16 keys]: x scale, log2 vs, 1/vs, page
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_meta + kKtMeta * 8);
   uint64_t* q_full = bars;
   uint64_t* slot_full = bars + 1;
@@ -211,8 +214,8 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
   uint64_t* s_full = slot_empty + NS;      // [tile]
   uint64_t* p_full = s_full + 2;
   uint64_t* o_full = p_full + 2;
-  uint64_t* meta_full = o_full + 2;        // [kKtMeta]
-  uint64_t* staged_full = meta_full + kKtMeta;                     // [converter warp][stage]
+  uint64_t* meta_full = o_full + 2;        // [batch % 4]
+  uint64_t* staged_full = meta_full + kKtMeta / kKtBatch;                     // [converter warp][stage]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(staged_full + kKtConvWarps * L::kStages);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -253,7 +256,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
       mbar_init(&p_full[t], 128);
       mbar_init(&o_full[t], 1);
     }
-    for (int s = 0; s < kKtMeta; ++s) mbar_init(&meta_full[s], kKtKeys / kKtUnit);
+    for (int s = 0; s < kKtMeta / kKtBatch; ++s) mbar_init(&meta_full[s], 1);
     for (int s = 0; s < kKtConvWarps * L::kStages; ++s) mbar_init(&staged_full[s], 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -283,88 +286,80 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
     const uint32_t seg_bytes = seg_keys * D;
     const uint32_t stage0 = smem_u32(staged + warp * L::kStages * L::kUnit);
     uint64_t* full = staged_full + warp * L::kStages;
-    auto unit_key = [&](int g) { return (blk0 + (g >> 2)) * kKtKeys + (g & 1) * kKtUnit; };
-    auto fetch_page = [&](int g, int in) {   // the page of the key `in` places into unit g
-      const int key = unit_key(g) + in;
-      return g < units && in < kKtUnit && key < len ? kv_page(p.c, b, key >> p.c.page_shift) : -1;
+    // Pages and scales are looked up for four blocks at a time, a lane for each 16 keys, two batches ahead, and in
+    // three steps a unit apart, so that no load is waited for.  Batch m is the affair of the warp that has the
+    // first unit of batch m - 2.  (Each warp looking up its own units' took 1400 cycles a unit.)
+    int look_page = -1;
+    float look_k = 0.0f, look_v = 0.0f;
+    auto look_pages = [&](int m) {
+      const int key = (blk0 + m * kKtBatch) * kKtKeys + 16 * lane;
+      look_page = -1;
+      if (16 * m < units && key < len) look_page = kv_page(p.c, b, key >> p.c.page_shift);
     };
-    auto issue = [&](int g, int stage, int page) {   // lane j copies segment j
+    auto look_scales = [&]() {
+      if (look_page >= 0) {
+        const int64_t ph = static_cast<int64_t>(look_page) * p.c.heads + hk;
+        look_k = p.c.scale[0][ph];
+        look_v = p.c.scale[1][ph];
+      }
+    };
+    auto write_meta = [&](int m) {
+      float4 f = make_float4(1.0f, -INFINITY, 0.0f, __int_as_float(-1));       // no page: weight 0
+      if (look_page >= 0) {   // a scale of zero: a page never written holds zeros
+        const float v = fmaxf(look_v, kKvMinScale);
+        const int poisoned = isnan(look_k) || isnan(look_v) ? kPoisoned : 0;
+        f = make_float4(fmaxf(look_k, kKvMinScale) * fabsf(p.scale_log2), log2f(v), __frcp_rn(v),
+                        __int_as_float(look_page | poisoned));
+      }
+      s_meta[(m * kKtBatch % kKtMeta) * 8 + lane] = f;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&meta_full[m % (kKtMeta / kKtBatch)]);
+    };
+    int known = -1;         // the last batch seen to be there
+    auto know = [&](int g) {
+      const int m = g >> 4;
+      if (m <= known) return true;
+      known = m;
+      return static_cast<bool>(__all_sync(0xffffffffu, mbar_wait(&meta_full[m % (kKtMeta / kKtBatch)],
+                                                                 (m / (kKtMeta / kKtBatch)) & 1, abort_flag)));
+    };
+    // what is known of the 16 keys `in` places into unit g
+    auto page_of = [&](int g, int in) {
+      return __float_as_int(s_meta[((g >> 2) % kKtMeta) * 8 + ((g & 1) * kKtUnit + in) / 16].w);
+    };
+    auto issue = [&](int g, int stage) {   // lane j copies segment j
+      const int page = lane < segs ? page_of(g, lane * seg_keys) : -1;
       const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
       if (lane == 0) mbar_arrive_expect_tx(&full[stage], seg_bytes * __popc(there));
       __syncwarp();
       if (page >= 0) {
-        const int key = unit_key(g) + lane * seg_keys;
-        const int64_t off = ((static_cast<int64_t>(page) * p.c.heads + hk) * p.c.page + (key & (p.c.page - 1))) * D;
+        const int key = (blk0 + (g >> 2)) * kKtKeys + (g & 1) * kKtUnit + lane * seg_keys;
+        const int64_t off =
+            ((static_cast<int64_t>(page & ~kPoisoned) * p.c.heads + hk) * p.c.page + (key & (p.c.page - 1))) * D;
         bulk_load(stage0 + stage * L::kUnit + lane * seg_bytes, p.c.code[(g >> 1) & 1] + off, seg_bytes,
                   smem_u32(&full[stage]));
       }
     };
-    auto next_k = [&](int g) {     // the warp's first K unit after g
-      do g += kKtConvWarps;
-      while (g < units && ((g >> 1) & 1));
-      return g;
-    };
-    // Global loads are asked for ahead and not looked at before they are needed, so that none is waited for:
-    // the page numbers of a unit's copies one unit before the copies, a K unit's scales two K units before
-    // their use (lanes 0..3: its four groups of 16 keys) and their page numbers three.
-    auto ask_page = [&](int key, bool want) {
-      const int slot = key >> p.c.page_shift;
-      return want && key < len && static_cast<unsigned>(slot) < static_cast<unsigned>(p.c.width)
-                 ? p.c.table[static_cast<int64_t>(b) * p.c.width + slot] : -1;
-    };
-    struct Scales {
-      float k, v;
-      bool have;
-    };
-    auto ask_k_page = [&](int g) { return ask_page(unit_key(g) + 16 * lane, lane < 4 && g < units); };
-    auto ask_scales = [&](int page) {
-      Scales r{0.0f, 0.0f, static_cast<unsigned>(page) < static_cast<unsigned>(p.c.num_pages)};
-      if (r.have) {
-        const int64_t ph = static_cast<int64_t>(page) * p.c.heads + hk;
-        r.k = p.c.scale[0][ph];
-        r.v = p.c.scale[1][ph];
-      }
-      return r;
-    };
-    auto seg_page = [&](int g) { return fetch_page(g, lane < segs ? lane * seg_keys : kKtUnit); };
-#pragma unroll
-    for (int st = 0; st < L::kStages; ++st)
-      if (warp + st * kKtConvWarps < units) issue(warp + st * kKtConvWarps, st, seg_page(warp + st * kKtConvWarps));
-    int k2 = (warp >> 1) & 1 ? next_k(warp) : warp;         // the K unit whose page is asked for last
-    Scales now = ask_scales(ask_k_page(k2));
-    k2 = next_k(k2);
-    Scales then = ask_scales(ask_k_page(k2));
-    k2 = next_k(k2);
-    int page_k = ask_k_page(k2);
-    int page_next = ask_page(unit_key(warp + L::kStages * kKtConvWarps) + lane * seg_keys,
-                             lane < segs && warp + L::kStages * kKtConvWarps < units);
+    if (warp < 2 && 16 * warp < units) {
+      look_pages(warp);
+      look_scales();
+      write_meta(warp);
+    }
     int stage = 0;
     uint32_t phase = 0;
-    bool ok = true;
+    bool ok = units == 0 || know(0);
+    int issued = 0;
+#pragma unroll 1
+    for (int st = 0; st < L::kStages; ++st)
+      if (ok && warp + st * kKtConvWarps < units) issue(warp + st * kKtConvWarps, st), ++issued;
     int g = warp;
-    for (; g < units; g += kKtConvWarps) {
+    for (; ok && g < units; g += kKtConvWarps) {
       const bool is_v = (g >> 1) & 1;
-      const int seq = g >> 1, j = g >> 2, s = seq % NS;
+      const int seq = g >> 1, s = seq % NS;
       const int after = g + L::kStages * kKtConvWarps;     // the unit that takes this stage next
-      // A page with a NaN scale gets NaN keys instead, so that it reaches the rows that see it and no other.
-      unsigned poisoned = 0;
-      if (!is_v) {
-        poisoned = __ballot_sync(0xffffffffu, now.have && (isnan(now.k) || isnan(now.v)));
-        if (lane < 4) {
-          float4 f = make_float4(1.0f, -INFINITY, 0.0f, 0.0f);       // no page: weight 0
-          if (now.have) {   // a scale of zero: a page never written holds zeros
-            const float v = fmaxf(now.v, kKvMinScale);
-            f = make_float4(fmaxf(now.k, kKvMinScale) * fabsf(p.scale_log2), log2f(v), __frcp_rn(v), 0.0f);
-          }
-          s_meta[(j % kKtMeta) * 8 + (g & 1) * 4 + lane] = f;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&meta_full[j % kKtMeta]);
-        now = then;
-        then = ask_scales(page_k);
-        k2 = next_k(k2);
-        page_k = ask_k_page(k2);
-      }
+      if ((g & 15) == 0) look_pages((g >> 4) + 2);
+      if ((g & 15) == 3) look_scales();
+      if ((g & 15) == 6 && 16 * ((g >> 4) + 2) < units) write_meta((g >> 4) + 2);
       ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, abort_flag) &&
                                        mbar_wait(&slot_empty[s], ((seq / NS) & 1) ^ 1, abort_flag));
       if (!ok) break;
@@ -402,45 +397,46 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
                        swap ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(h[4], h[5], h[6], h[7]));
         }
       }
-      if (poisoned) {
-        const uint4 nan = make_uint4(0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u);
+      // A page with a NaN scale gets NaN keys instead, so that it reaches the rows that see it and no other.
+      if (!is_v) {
+        const int page = lane < 4 ? page_of(g, 16 * lane) : -1;
+        const unsigned poisoned = __ballot_sync(0xffffffffu, page >= kPoisoned);
+        if (poisoned) {
+          const uint4 nan = make_uint4(0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u);
 #pragma unroll 1
-        for (int i = 0; i < kVecs; ++i)
-          if (poisoned >> (i * 4 / kVecs) & 1u) {
-            const int r = (key_in + i * kKeyStep) & 7;
-            st_shared_v4(dst + i * kKeyStep * 128 + (((2 * (col & 3)) ^ r) << 4), nan);
-            st_shared_v4(dst + i * kKeyStep * 128 + (((2 * (col & 3) + 1) ^ r) << 4), nan);
-          }
+          for (int i = 0; i < kVecs; ++i)
+            if (poisoned >> (i * 4 / kVecs) & 1u) {
+              const int r = (key_in + i * kKeyStep) & 7;
+              st_shared_v4(dst + i * kKeyStep * 128 + (((2 * (col & 3)) ^ r) << 4), nan);
+              st_shared_v4(dst + i * kKeyStep * 128 + (((2 * (col & 3) + 1) ^ r) << 4), nan);
+            }
+        }
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&slot_full[s]);
       if (after < units) {
-        if (static_cast<unsigned>(page_next) >= static_cast<unsigned>(p.c.num_pages)) {
-          if (lane < segs && unit_key(after) + lane * seg_keys < len) record_error(kErrKvPage);
-          page_next = -1;
-        }
-        issue(after, stage, page_next);
-        page_next = ask_page(unit_key(after + kKtConvWarps) + lane * seg_keys,
-                             lane < segs && after + kKtConvWarps < units);
+        ok = know(after);
+        if (ok) issue(after, stage);
       }
       if (++stage == L::kStages) stage = 0, phase ^= 1;
     }
-    if (!ok) {   // let the copies in flight land before the block's memory goes
-      for (int st = 1; st < L::kStages; ++st) {
-        if (++stage == L::kStages) stage = 0, phase ^= 1;
-        if (g + st * kKtConvWarps < units) mbar_wait(&full[stage], phase, nullptr);
+    if (!ok) {   // a wait gave up: let every copy in flight land before the block's memory goes
+      for (int st = 0; st < L::kStages; ++st) {
+        const int last = g + st * kKtConvWarps;      // units g .. are the ones that may be in flight
+        if (last < units && st < issued) mbar_wait(&full[(stage + st) % L::kStages], phase ^ (stage + st >= L::kStages ? 1u : 0u), nullptr);
       }
     }
   } else if (warp == 3) {
     // ------------------------------- MMA issuer -------------------------------
     if (elect_one_sync()) {
+      constexpr bool kEarly = NS >= 5;
       constexpr uint32_t idesc_qk = make_idesc_f16(kKtRows, kKtKeys);
       constexpr uint32_t idesc_pv = make_idesc_f16(kKtRows, D) | (1u << 16);   // V is MN-major
       bool ok = n_blocks == 0 || mbar_poll(q_full, 0, abort_flag);
       auto issue_s = [&](int j, int t) -> bool {
         const int seq = 2 * j, s = seq % NS;
-        if (t == 0 && !mbar_poll(&slot_full[s], (seq / NS) & 1, abort_flag)) return false;
+        if (!kEarly && t == 0 && !mbar_poll(&slot_full[s], (seq / NS) & 1, abort_flag)) return false;
         tc_fence_after();
         const uint32_t qb = smem_u32(sq + t * L::kTile), kb = smem_u32(ring + s * L::kTile);
 #pragma unroll
@@ -451,10 +447,13 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
         if (t == tiles - 1) tc_commit(&slot_empty[s]);
         return true;
       };
+      auto have = [&](int seq) { return mbar_poll(&slot_full[seq % NS], (seq / NS) & 1, abort_flag); };
+      if (kEarly && n_blocks > 0) ok = ok && have(0);
       for (int t = 0; t < tiles && ok && n_blocks > 0; ++t) ok = issue_s(0, t);
       for (int j = 0; j < n_blocks && ok; ++j) {
         const int seq = 2 * j + 1, s = seq % NS;
-        if (!mbar_poll(&slot_full[s], (seq / NS) & 1, abort_flag)) break;
+        // V(j), and where the ring is deep enough for it K(j + 1), before the weights: off the tiles' chain
+        if (!have(seq) || (kEarly && j + 1 < n_blocks && !have(seq + 1))) break;
         for (int t = 0; t < tiles && ok; ++t) {
           if (!mbar_poll(&p_full[t], j & 1, abort_flag)) { ok = false; break; }
           tc_fence_after();
@@ -515,8 +514,12 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
       }
       float m = -INFINITY, l = 0.0f;
       bool ok = true;
+      auto wait_meta = [&](int m) {
+        ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(smem_u32(&meta_full[m % (kKtMeta / kKtBatch)]),
+                                                         (m / (kKtMeta / kKtBatch)) & 1, abort_flag));
+      };
+      if (n_blocks > 0) wait_meta(0);
       for (int j = 0; j < n_blocks; ++j) {
-        ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(smem_u32(&meta_full[j % kKtMeta]), (j / kKtMeta) & 1, abort_flag));
         // S(j) is there, and with it everything issued before: O holds W V up to block j - 1
         ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(smem_u32(&s_full[tile]), j & 1, abort_flag));
         uint32_t meta = smem_u32(s_meta + (j % kKtMeta) * 8);
@@ -550,6 +553,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
         tmem_st_wait();
         tc_fence_before();
         if (ok) mbar_arrive(&p_full[tile]);
+        if (j + 1 < n_blocks && (j + 1) % kKtBatch == 0) wait_meta((j + 1) / kKtBatch);      // under the next products
       }
       if (n_blocks > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(smem_u32(&o_full[tile]), 0, abort_flag));
       const bool have = ok && n_blocks > 0;
