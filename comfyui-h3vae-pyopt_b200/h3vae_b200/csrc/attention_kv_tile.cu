@@ -201,6 +201,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const KvAttnParams p) {
   using L = KvTile<D>;
   constexpr int NS = L::kSlots;
+  constexpr uint32_t kWCol = D == 64 ? 192 : 0;     // the weights' columns of a row tile: O takes 128 .. 128 + D
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sq = smem;
@@ -430,13 +431,12 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
   } else if (warp == 3) {
     // ------------------------------- MMA issuer -------------------------------
     if (elect_one_sync()) {
-      constexpr bool kEarly = NS >= 5;
       constexpr uint32_t idesc_qk = make_idesc_f16(kKtRows, kKtKeys);
       constexpr uint32_t idesc_pv = make_idesc_f16(kKtRows, D) | (1u << 16);   // V is MN-major
       bool ok = n_blocks == 0 || mbar_poll(q_full, 0, abort_flag);
-      auto issue_s = [&](int j, int t) -> bool {
-        const int seq = 2 * j, s = seq % NS;
-        if (!kEarly && t == 0 && !mbar_poll(&slot_full[s], (seq / NS) & 1, abort_flag)) return false;
+      auto have = [&](int seq) { return mbar_poll(&slot_full[seq % NS], (seq / NS) & 1, abort_flag); };
+      auto issue_s = [&](int j, int t) {
+        const int s = (2 * j) % NS;
         tc_fence_after();
         const uint32_t qb = smem_u32(sq + t * L::kTile), kb = smem_u32(ring + s * L::kTile);
 #pragma unroll
@@ -445,17 +445,21 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
                   make_sw128_desc(kb + (k >> 2) * 16384) + 2 * (k & 3), idesc_qk, k > 0 ? 1u : 0u);
         tc_commit(&s_full[t]);
         if (t == tiles - 1) tc_commit(&slot_empty[s]);
-        return true;
       };
-      auto have = [&](int seq) { return mbar_poll(&slot_full[seq % NS], (seq / NS) & 1, abort_flag); };
-      if (kEarly && n_blocks > 0) ok = ok && have(0);
-      for (int t = 0; t < tiles && ok && n_blocks > 0; ++t) ok = issue_s(0, t);
+      if (n_blocks > 0) {
+        ok = ok && have(0);
+        for (int t = 0; t < tiles && ok; ++t) issue_s(0, t);
+      }
       for (int j = 0; j < n_blocks && ok; ++j) {
-        const int seq = 2 * j + 1, s = seq % NS;
-        // V(j), and where the ring is deep enough for it K(j + 1), before the weights: off the tiles' chain
-        if (!have(seq) || (kEarly && j + 1 < n_blocks && !have(seq + 1))) break;
+        const int s = (2 * j + 1) % NS;
+        // what is not there yet is waited for before the weights, off the tiles' chain, where the ring is deep enough
+        ok = have(2 * j + 1) && (kWCol == 0 || j + 1 == n_blocks || have(2 * j + 2));
         for (int t = 0; t < tiles && ok; ++t) {
           if (!mbar_poll(&p_full[t], j & 1, abort_flag)) { ok = false; break; }
+          // Dim 64 has columns for the weights beside the products', so the next products, which the softmax waits
+          // for, go first.  Dim 128 has the weights where they go: they wait until these are used (nothing orders
+          // products of different accumulators).
+          if (kWCol != 0 && j + 1 < n_blocks) issue_s(j + 1, t);
           tc_fence_after();
           const uint32_t vb = smem_u32(ring + s * L::kTile);
 #pragma unroll
@@ -463,12 +467,14 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
             // 64 dims of 16 keys are one swizzle atom column; the next 64 dims lie 16 KB further
             uint64_t vd = make_sw128_desc(vb + k * 16 * 128);
             vd = (vd & ~(uint64_t(0x3FFFu) << 16)) | (uint64_t(16384 >> 4) << 16);
-            mma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, vd, idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
+            mma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + kWCol + 8 * k, vd, idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
           }
-          if (j + 1 == n_blocks) tc_commit(&o_full[t]);
+          tc_commit(&o_full[t]);
           if (t == tiles - 1) tc_commit(&slot_empty[s]);
-          // The next products go where the weights were: the tensor core takes its instructions in order.
-          if (j + 1 < n_blocks) ok = issue_s(j + 1, t);
+          if (kWCol == 0 && j + 1 < n_blocks) {
+            ok = (t > 0 || have(2 * j + 2)) && mbar_poll(&o_full[t], j & 1, abort_flag);
+            if (ok) issue_s(j + 1, t);
+          }
         }
       }
     }
@@ -520,7 +526,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
       };
       if (n_blocks > 0) wait_meta(0);
       for (int j = 0; j < n_blocks; ++j) {
-        // S(j) is there, and with it everything issued before: O holds W V up to block j - 1
+        // (dim 128: S(j) was issued after W V of block j - 1 was done, so O is whole)
         ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(smem_u32(&s_full[tile]), j & 1, abort_flag));
         uint32_t meta = smem_u32(s_meta + (j % kKtMeta) * 8);
         asm volatile("" : "+r"(meta));     // its loads stay below the wait
@@ -547,15 +553,21 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
           if (look || !__any_sync(0xffffffffu, most > kKtMostWeight)) break;
           look = true;
         }
-        tmem_st64(t_s, w);      // over the products that they came from
         l = __fmaf_rn(l, alpha, sum);
-        if (j > 0 && __any_sync(0xffffffffu, moved)) rescale_row(t_o, D, alpha);
+        // W V of block j - 1 is done: its weights' columns are free, and O is whole
+        if (kWCol != 0 && j > 0)
+          ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(smem_u32(&o_full[tile]), (j - 1) & 1, abort_flag));
+        tmem_st64(t_s + kWCol, w);      // dim 128: over the products that they came from
+        if (j > 0 && __any_sync(0xffffffffu, moved)) {
+          tc_fence_after();
+          rescale_row(t_o, D, alpha);
+        }
         tmem_st_wait();
         tc_fence_before();
         if (ok) mbar_arrive(&p_full[tile]);
         if (j + 1 < n_blocks && (j + 1) % kKtBatch == 0) wait_meta((j + 1) / kKtBatch);      // under the next products
       }
-      if (n_blocks > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(smem_u32(&o_full[tile]), 0, abort_flag));
+      if (n_blocks > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(smem_u32(&o_full[tile]), (n_blocks - 1) & 1, abort_flag));
       const bool have = ok && n_blocks > 0;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       if (have) tc_fence_after();
