@@ -78,7 +78,7 @@ template <typename T, int VPT, int kThreads>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvWriteParams p) {
   constexpr int kWarps = kThreads / 32;
   __shared__ uint32_t s_max[kWarps];
-  __shared__ int s_sum[kWarps][128];
+  __shared__ __align__(16) uint32_t s_sum[kWarps][64];
   const int kv = blockIdx.x & 1, head = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const int count = p.counts ? min(p.counts[b], p.tokens) : p.tokens;
   const int start = p.start[b];
@@ -93,15 +93,17 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvWriteParams 
   const int hi = static_cast<int>(min(end - page_begin, static_cast<int64_t>(p.c.page)));       // past the last one
   if (hi <= lo) return;
 
-  // the new rows are asked for before the page is looked up
-  const int chunk_shift = p.dim == 64 ? 3 : 4;
+  // the new rows are asked for before the page is looked up; a thread's vectors lie kThreads apart, in one column
+  const int chunk_shift = p.dim == 64 ? 3 : 4, row_step = kThreads >> chunk_shift;
+  const int row0 = tid >> chunk_shift;
   const T* src = static_cast<const T*>(p.x[kv]) + b * p.stride[kv][0] + head * p.stride[kv][1] +
-                 (page_begin - start) * p.stride[kv][2];
+                 (page_begin - start + row0) * p.stride[kv][2] + (tid & ((1 << chunk_shift) - 1)) * 8;
+  const int64_t src_step = row_step * p.stride[kv][2];
   KvRaw<T> x[VPT];
 #pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    const int i = tid + j * kThreads, row = i >> chunk_shift, col = (i & ((1 << chunk_shift) - 1)) * 8;
-    if (row >= lo && row < hi) x[j].load(src + row * p.stride[kv][2] + col, p.vec[kv]);
+  for (int j = 0; j < VPT; ++j, src += src_step) {
+    const int row = row0 + j * row_step;
+    if (row >= lo && row < hi) x[j].load(src, p.vec[kv]);
     else x[j].zero();
   }
   const int page = kv_page(p.c, b, slot);
@@ -126,11 +128,12 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvWriteParams 
   const bool grown = lo > 0 && s > old_scale;
   const bool complete = kv == 0 && hi == p.c.page;
   const float inv = __frcp_rn(s), ratio = __fdiv_rn(old_scale, s);
-  int sum[8] = {};
+  // Column sums of codes + 128, two to a word: at most 128 rows of 255 fit 16 bits.
+  uint32_t sum[4] = {};      // codes 0 and 2, 1 and 3, 4 and 6, 5 and 7 of the column's eight
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
-    const int i = tid + j * kThreads, row = i >> chunk_shift;
-    uint2* at = reinterpret_cast<uint2*>(codes) + i;
+    const int row = row0 + j * row_step;
+    uint2* at = reinterpret_cast<uint2*>(codes) + tid + j * kThreads;
     uint2 w = make_uint2(0u, 0u);
     bool store = false;
     if (row >= lo && row < hi) {
@@ -138,10 +141,7 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvWriteParams 
       if (!lost) {   // |x * inv| <= 127 * (1 + 2^-22): no clamp is needed after rounding
         float f[8];
         x[j].values(f);
-        uint32_t q[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) q[e] = rint_bits(__fmul_rn(f[e], inv));
-        w = make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+        w = quantise8(f, inv);
       }
     } else if (row < lo && (grown || complete)) {
       w = *at;
@@ -150,40 +150,40 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvWriteParams 
         float f[8];
         codes_to_f32(w.x, f);
         codes_to_f32(w.y, f + 4);
-        uint32_t q[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) q[e] = rint_bits(__fmul_rn(f[e], ratio));
-        w = make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+        w = quantise8(f, ratio);
       }
     }
     if (store) *at = w;
     if (complete) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] += static_cast<int8_t>((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
+      const uint32_t a = w.x ^ 0x80808080u, c = w.y ^ 0x80808080u;
+      sum[0] += a & 0x00ff00ffu;
+      sum[1] += (a >> 8) & 0x00ff00ffu;
+      sum[2] += c & 0x00ff00ffu;
+      sum[3] += (c >> 8) & 0x00ff00ffu;
     }
   }
   if (tid == 0) *scale_at = lost ? __int_as_float(0x7fffffff) : s;
   if (complete) {
-    // a thread's vectors share their column (the thread count is a multiple of the vectors in a row)
     const int chunks = 1 << chunk_shift;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < 4; ++e)
       for (int o = chunks; o < 32; o <<= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
-    if ((tid & 31) < chunks) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s_sum[tid >> 5][(tid & 31) * 8 + e] = sum[e];
-    }
+    if ((tid & 31) < chunks)
+      *reinterpret_cast<uint4*>(&s_sum[tid >> 5][(tid & 31) * 4]) = make_uint4(sum[0], sum[1], sum[2], sum[3]);
     __syncthreads();
     if (tid < p.dim) {
+      // dim tid: word (tid / 8) * 4 + its place in the order above, low or high half
+      const int in = tid & 7, word = (tid >> 3) * 4 + (in >> 2) * 2 + (in & 1), shift = (in & 2) * 8;
       int t = 0;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) t += s_sum[w][tid];
-      p.c.k_sum[ph * p.dim + tid] = static_cast<int16_t>(t);
+      for (int w = 0; w < kWarps; ++w) t += static_cast<int>((s_sum[w][word] >> shift) & 0xffffu);
+      p.c.k_sum[ph * p.dim + tid] = static_cast<int16_t>(t - 128 * p.c.page);
     }
   }
 }
 
-// Read: one thread per 8 codes of K and of V (8 B in, 16 B out of fp16 each).
+// Read: a thread takes 8 codes of K and of V (8 B in, 16 B out of fp16 each) of
+// kKvReadRows rows, so that several loads are on their way.
 struct KvReadParams {
   KvView c;
   const int32_t* start;
@@ -193,37 +193,52 @@ struct KvReadParams {
 };
 
 constexpr int kKvReadThreads = 256;
+constexpr int kKvReadRows = 2;
 
 template <typename T>
 __global__ void __launch_bounds__(kKvReadThreads) kv_read_kernel(const KvReadParams p) {
   const int head = blockIdx.y, b = blockIdx.z;
-  const int i = blockIdx.x * kKvReadThreads + threadIdx.x;
-  const int row = i >> p.chunk_shift, col = (i & ((1 << p.chunk_shift) - 1)) * 8;
-  if (row >= p.tokens) return;
-  const int dim = 8 << p.chunk_shift;
-  const int64_t pos = static_cast<int64_t>(p.start ? p.start[b] : 0) + row;
-  int page = -1;
-  if (pos >= 0 && pos < p.lengths[b]) page = kv_page(p.c, b, static_cast<int>(pos >> p.c.page_shift));
-  const int64_t ph = static_cast<int64_t>(page) * p.c.heads + head;
-  const int64_t from = (ph * p.c.page + (pos & (p.c.page - 1))) * dim + col;
-  const int64_t to = ((static_cast<int64_t>(b) * p.c.heads + head) * p.tokens + row) * dim + col;
+  const int dim = 8 << p.chunk_shift, step = kKvReadThreads >> p.chunk_shift;
+  const int row0 = blockIdx.x * step * kKvReadRows + (threadIdx.x >> p.chunk_shift);
+  const int col = (threadIdx.x & ((1 << p.chunk_shift) - 1)) * 8;
+  const int64_t first = p.start ? p.start[b] : 0, len = p.lengths[b];
+  uint2 w[kKvReadRows][2];
+  float s[kKvReadRows][2];
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    float x[8] = {};
-    if (page >= 0) {
-      const uint2 w = *reinterpret_cast<const uint2*>(p.c.code[kv] + from);
-      const float s = p.c.scale[kv][ph];
-      codes_to_f32(w.x, x);
-      codes_to_f32(w.y, x + 4);
+  for (int r = 0; r < kKvReadRows; ++r) {
+    const int row = row0 + r * step;
+    const int64_t pos = first + row;
+    const int page = row < p.tokens && pos >= 0 && pos < len ? kv_page(p.c, b, static_cast<int>(pos >> p.c.page_shift)) : -1;
+    const int64_t ph = static_cast<int64_t>(page) * p.c.heads + head;
+    const int64_t from = (ph * p.c.page + (pos & (p.c.page - 1))) * dim + col;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(x[e], s);
+    for (int kv = 0; kv < 2; ++kv) {
+      w[r][kv] = make_uint2(0u, 0u);
+      s[r][kv] = 0.0f;
+      if (page >= 0) {
+        w[r][kv] = *reinterpret_cast<const uint2*>(p.c.code[kv] + from);
+        s[r][kv] = p.c.scale[kv][ph];
+      }
     }
-    __align__(16) T y[8];
+  }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) from_f32(x[e], y[e]);
-    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out[kv]) + to);
+  for (int r = 0; r < kKvReadRows; ++r) {
+    const int row = row0 + r * step;
+    if (row >= p.tokens) return;
+    const int64_t to = ((static_cast<int64_t>(b) * p.c.heads + head) * p.tokens + row) * dim + col;
 #pragma unroll
-    for (int k = 0; k < KvVec8<T>::kWords / 4; ++k) dst[k] = reinterpret_cast<const uint4*>(y)[k];
+    for (int kv = 0; kv < 2; ++kv) {
+      float x[8];
+      codes_to_f32(w[r][kv].x, x);
+      codes_to_f32(w[r][kv].y, x + 4);
+      scale8(x, s[r][kv]);
+      __align__(16) T y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) from_f32(x[e], y[e]);
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out[kv]) + to);
+#pragma unroll
+      for (int k = 0; k < KvVec8<T>::kWords / 4; ++k) dst[k] = reinterpret_cast<const uint4*>(y)[k];
+    }
   }
 }
 
@@ -301,9 +316,8 @@ extern "C" int h3b_kv_read_i8(const h3b_kv_cache* cache, const int32_t* page_tab
   p.out[1] = v;
   p.tokens = (int)tokens;
   p.chunk_shift = cache->head_dim == 64 ? 3 : 4;
-  const int64_t vecs = tokens << p.chunk_shift;
-  dim3 grid((unsigned)((vecs + h3b::kKvReadThreads - 1) / h3b::kKvReadThreads), (unsigned)cache->kv_heads,
-            (unsigned)batch);
+  const int64_t rows = (int64_t)(h3b::kKvReadThreads >> p.chunk_shift) * h3b::kKvReadRows;
+  dim3 grid((unsigned)((tokens + rows - 1) / rows), (unsigned)cache->kv_heads, (unsigned)batch);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == H3B_TYPE_F16) h3b::kv_read_kernel<__half><<<grid, h3b::kKvReadThreads, 0, st>>>(p);
   else if (dtype == H3B_TYPE_BF16) h3b::kv_read_kernel<__nv_bfloat16><<<grid, h3b::kKvReadThreads, 0, st>>>(p);

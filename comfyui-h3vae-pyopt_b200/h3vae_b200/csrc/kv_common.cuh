@@ -74,12 +74,33 @@ __device__ __forceinline__ void codes_to_f32(uint32_t w, float* x) {
     x[i] = __fsub_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + i)), 8388736.0f);
 }
 
+// Eight products with `f`, each rounded to nearest: packed fp32 pairs round each
+// lane like the scalar operation.
+__device__ __forceinline__ void scale8(float (&x)[8], float f) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float2 y = f2x_mul(make_float2(x[e], x[e + 1]), make_float2(f, f));
+    x[e] = y.x;
+    x[e + 1] = y.y;
+  }
+}
+
 // The low byte of rint(x) for |x| < 2^21 sits in the low mantissa byte of
 // x + 1.5 * 2^23 (two's complement, ties to even).
 __device__ __forceinline__ uint32_t rint_bits(float x) { return __float_as_uint(__fadd_rn(x, 12582912.0f)); }
 
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// rint(x * f) of eight values as bytes, |x * f| < 2^21: the product rounded to
+// nearest, then to an integer by the addition of rint_bits.
+__device__ __forceinline__ uint2 quantise8(float (&x)[8], float f) {
+  scale8(x, f);
+  uint32_t q[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) q[e] = rint_bits(x[e]);   // scalar: with the packed addition, codes differed (the pair was fused)
+  return make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
 }
 
 }  // namespace h3b
