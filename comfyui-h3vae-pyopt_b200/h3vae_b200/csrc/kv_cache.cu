@@ -4,10 +4,15 @@
 //   a = max|x|;  s = max(a * fp32(1/127), 1e-30), and max(s, old scale) when the
 //   page keeps earlier tokens, whose codes become rint(code * (old / s)) if s
 //   grew;  code = rint(x * (1/s)).
-// One CTA per (page slot, head, K or V): the page's new values (at most 16 KB
+// One CTA per (page slot, head, K or V): the page's new values (at most 32 KB
 // of fp16) stay in registers between the maximum and the quantisation, so every
-// input is read once and every code written once.  Bound: HBM, 2 B read and
-// 1 B written per element.
+// input is read once and every code written once.  They stay as they came, in 16
+// bits (as fp32 a 128 x 128 page took 128 registers a thread and 250 us where it
+// now takes 52), and are asked for before the page number is known.  Bound: HBM,
+// 2 B read and 1 B written per element, and the ~6 instructions an element takes:
+// 4 x 16 heads x 5120 tokens of dim 64, fp16, 126 MB in 26.7 us = 4.7 TB/s; bf16
+// prompts of up to 16001 tokens, 8 heads of dim 128, 52 us.  A single token per
+// sequence is a launch: 3.4 us.
 #include <cstring>
 
 #include "kv_common.cuh"
@@ -183,7 +188,9 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const KvWriteParams 
 }
 
 // Read: a thread takes 8 codes of K and of V (8 B in, 16 B out of fp16 each) of
-// kKvReadRows rows, so that several loads are on their way.
+// kKvReadRows rows, so that several loads are on their way.  Bound: HBM.  8 x up
+// to 32768 tokens, 8 heads of dim 128, bf16: 222 us = 6.4 TB/s (250 with one
+// product at a time, 241 with four rows, 225 with one).
 struct KvReadParams {
   KvView c;
   const int32_t* start;
