@@ -57,8 +57,8 @@ KvPlan kv_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens,
   // which are as many for every row; long sequences of different lengths are better cut into equal parts
   // (16 x 6553..32768 keys: 154 us in clusters of eight, 140 in parts).
   const int64_t wave = kSplitBlocks * h3b_host::num_sms();
-  int64_t c = 1;
-  while (c < kSplitCluster && 2 * c * items <= wave && c * kSplitWarps < tiles) c *= 2;
+  const int64_t c = std::max<int64_t>(
+      1, std::min({(int64_t)kSplitCluster, wave / items, (tiles + kSplitWarps - 1) / kSplitWarps}));
   if ((tiles + c - 1) / c <= most && (tiles <= c * kSplitWarps * 4 || (n_selected > 0 && c * items >= wave / 2))) {
     k.cluster = c;
     k.slots = c;
