@@ -24,7 +24,7 @@ constexpr int64_t kTileBytes = int64_t(24) << 20;
 // per query token).
 struct KvPlan {
   bool tile;
-  int64_t row_tiles, slots, chunk, target, cluster;
+  int64_t row_tiles, slots, chunk, share, fit, cluster, join_warps;
   size_t plan_bytes, part_bytes;
 };
 
@@ -32,6 +32,7 @@ KvPlan kv_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens,
                int64_t page, int64_t n_selected) {
   using namespace h3b;
   KvPlan k{};
+  k.join_warps = 1;
   const int64_t group = q_heads / kv_heads;
   const int64_t keys = kSplitStageBytes / 2 / dim;
   const int64_t most = (kSplitPages - 1) * page / keys;    // tiles a run may have: it may start inside a page
@@ -44,18 +45,16 @@ KvPlan kv_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens,
     const int64_t blocks = batch * kv_heads * k.row_tiles, most_blocks = (width * page + kKtKeys - 1) / kKtKeys;
     k.slots = std::max<int64_t>(1, std::min(h3b_host::num_sms() / blocks, most_blocks / 4));
     k.part_bytes = k.slots > 1 ? (size_t)(k.slots * batch * kv_heads * rows) * (dim + 4) * 4 : 0;
+    k.join_warps = k.slots >= 4 ? 4 : 1;
     return k;
   }
   k.row_tiles = row_tiles;
-  // one wave of blocks over selected pages, two over ragged lengths (measured on 16 x 48 pages: 27, 29, 32 us for
-  // one, two, three; on 16 x 6553..32768 keys: 158, 139, 139)
-  k.target = (n_selected > 0 ? 1 : 2) * kSplitBlocks * h3b_host::num_sms();
   const int64_t items = batch * kv_heads * k.row_tiles * (n_selected > 0 ? tokens : 1);
   const int64_t tiles = ((n_selected > 0 ? n_selected : width) * page + keys - 1) / keys;
   // Up to eight runs of a row tile's keys join inside a cluster: one launch and no trip through global memory
   // (one token over 1797 keys, 16 heads: 6.5 us, 8.6 with a second kernel).  For short runs, and for selected pages,
   // which are as many for every row; long sequences of different lengths are better cut into equal parts
-  // (16 x 6553..32768 keys: 154 us in clusters of eight, 140 in parts).
+  // (16 x 6553..32768 keys: 154 us in clusters of eight, 129 in parts).
   const int64_t wave = kSplitBlocks * h3b_host::num_sms();
   const int64_t c = std::max<int64_t>(
       1, std::min({(int64_t)kSplitCluster, wave / items, (tiles + kSplitWarps - 1) / kSplitWarps}));
@@ -67,15 +66,28 @@ KvPlan kv_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens,
   }
   // Few rows over long runs: parts through the workspace, joined by a second kernel.
   if (n_selected > 0) {
-    const int64_t want = std::max<int64_t>(1, std::min(k.target / items, (tiles + kSplitWarps - 1) / kSplitWarps));
+    const int64_t want = std::max<int64_t>(1, std::min(wave / items, (tiles + kSplitWarps - 1) / kSplitWarps));
     k.chunk = std::min(most, (tiles + want - 1) / want);
     k.slots = (tiles + k.chunk - 1) / k.chunk;
+    k.join_warps = k.slots >= 4 ? 4 : 1;
     k.part_bytes = k.slots > 1 ? (size_t)(batch * tokens * k.slots) * kv_heads * k.row_tiles * kSplitRows * (dim + 4) * 4 : 0;
   } else {
     k.chunk = most;
-    const int64_t more = std::min(k.target / (kv_heads * k.row_tiles), batch * ((tiles + kSplitWarps - 1) / kSplitWarps));
-    k.slots = batch + std::max(more, batch * (tiles / most));
+    const int64_t per = kv_heads * k.row_tiles;
+    const int64_t most_runs = batch * ((tiles + kSplitWarps - 1) / kSplitWarps);
+    // Runs fill whole waves of blocks exactly, as few as leave every row tile a few runs: the last wave of a count that
+    // fits none is nearly empty, and every run costs the join.  Measured, us for one, two, three waves (140, 50, 80, 217
+    // with 2 x wave + batch runs), 8 heads, dim 128: 16 x 6553..32768 keys 135, 129, 133; 1 x 32768 25, 33, 38; 7 x .. 65,
+    // 71, 80; 28 x .. 245, 215, 206.  More row tiles than blocks: equal runs of three waves' share, sequences not
+    // fitted (64 x 8192: 134, fitted 138); than two waves': only what is longer than a block's share of one is cut
+    // (200 x 4096: 195, cut to a third 213, nothing cut 190).
+    const bool many = items > wave;
+    const int64_t waves = many ? (items > 2 * wave ? 1 : 3) : items * 2 > wave ? 3 : items * 4 > wave ? 2 : 1;
+    k.share = std::max<int64_t>(1, std::min(waves * wave / per, most_runs));
+    k.fit = many ? batch + k.share : k.share;
+    k.slots = std::max(k.fit, batch + batch * (tiles / most));
     k.plan_bytes = k.slots > batch ? ((size_t)batch * 8 + 15) & ~size_t(15) : 0;
+    k.join_warps = k.slots >= 4 * batch ? 4 : 1;   // 56 parts of a row: the call takes 60 us with four, 75 with one
     k.part_bytes = k.slots > batch ? (size_t)k.slots * kv_heads * k.row_tiles * kSplitRows * (dim + 4) * 4 : 0;
   }
   return k;
@@ -99,7 +111,8 @@ template <typename T, int D, h3b::KvParts kParts>
 int launch_kv_join(const char* name, const h3b::KvAttnParams& p, int64_t batch, cudaStream_t st) {
   using namespace h3b;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(((int64_t)p.group * p.tokens + 3) / 4), (unsigned)p.c.heads, (unsigned)batch);
+  const int64_t a_block = 4 / p.join_warps;   // rows
+  cfg.gridDim = dim3((unsigned)(((int64_t)p.group * p.tokens + a_block - 1) / a_block), (unsigned)p.c.heads, (unsigned)batch);
   cfg.blockDim = dim3(128);
   cfg.stream = st;
   cudaLaunchAttribute attr{};   // the join's blocks may be resident before the parts are done; they wait for them
@@ -225,7 +238,9 @@ extern "C" int h3b_attention_kv_i8(const void* q, const int64_t* q_strides, cons
   p.scale_log2 = scale * h3b::kLog2e;
   p.row_tiles = (int)k.row_tiles;
   p.slots = (int)k.slots;
-  p.target = (int)k.target;
+  p.share = (int)k.share;
+  p.fit = (int)k.fit;
+  p.join_warps = (int)k.join_warps;
   p.chunk = (int)k.chunk;
   p.cluster = (int)k.cluster;
   p.plan = k.plan_bytes ? static_cast<int2*>(workspace) : nullptr;

@@ -31,7 +31,9 @@ struct KvAttnParams {
   bool causal, vec_q, vec_out;
   float scale_log2;
   // split plan (see attention_kv_split_kernel)
-  int row_tiles, slots, target, chunk;
+  int row_tiles, slots, chunk;
+  int share, fit;  // runs of keys per (kv head, row tile): as many as that many equal ones, at most so many in all
+  int join_warps;  // warps that join a row's parts: 1 or 4
   int cluster;     // > 0: the slots of a row tile are one cluster, which joins them itself
   float* part;     // [slot, kv head, row tile, row] x (dim + 2): weighted codes, m, l
   int2* plan;      // per sequence: first slot, number of slots

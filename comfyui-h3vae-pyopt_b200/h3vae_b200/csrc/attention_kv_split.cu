@@ -31,13 +31,13 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
 // The rows see nearly all keys of their sequence, so a call moves the cache's
 // bytes once and is bound by HBM when it is long and by latency (table, scale
 // and code loads in a row, then the join) when it is short.  One token each over
-// 16 x 6553..32768 keys, 8 heads of dim 128, 32 query heads: 690 MB in 141 us =
-// 4.9 TB/s, with the issue slots 52 % and the tensor pipe 30 % in use; 12 warps an
-// SM hide each other's latency (8 warps: 154 us; tiles of half the size 165 us,
-// of twice the size 178 us).  One token over 1797 keys of 16 heads: 6.5 us.
+// 16 x 6553..32768 keys, 8 heads of dim 128, 32 query heads: 690 MB in 129 us =
+// 5.3 TB/s, with the issue slots 56 % and the tensor pipe 32 % in use; 12 warps an
+// SM hide each other's latency.  Before runs were fitted to waves, at 141 us: 8 warps
+// 154 us, tiles of half the size 165 us, of twice the size 178 us.  One token over 1797 keys of 16 heads: 6.5 us.
 constexpr int kSplitWarps = 4;
 constexpr int kSplitStages = 2;
-constexpr int kSplitBlocks = 3;       // blocks an SM holds (two with three stages: 154 against 139 us on 16 x 32768 keys)
+constexpr int kSplitBlocks = 3;       // blocks an SM holds (two with three stages: 154 against 141 us on 16 x 6553..32768 keys)
 constexpr int kSplitCluster = 8;      // most blocks that join through shared memory
 constexpr int kSplitRows = 16;
 constexpr int kSplitPages = 256;      // pages a block's run of tiles may span
@@ -70,7 +70,6 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_s
   float4* s_meta = reinterpret_cast<float4*>(smem + S::kRing);                 // per page: x scale, log2 vs, 1/vs
   int* s_page = reinterpret_cast<int*>(s_meta + kSplitPages);                  // pool page, -1: none
   uint64_t* s_bar = reinterpret_cast<uint64_t*>(s_page + kSplitPages);
-  int* s_red = reinterpret_cast<int*>(s_bar + kSplitWarps * kSplitStages);     // 4 ints
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
   const int hk = blockIdx.y;
@@ -102,59 +101,86 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_s
     rt = blockIdx.x / p.slots;
     slot = blockIdx.x % p.slots;
     int t0, chunk, first_slot;
-    auto chunk_of = [&](int sum) {   // equal chunks of tiles for the whole batch
-      const int64_t total = static_cast<int64_t>(sum) * p.c.heads * p.row_tiles;
-      return static_cast<int>(min(max((total + p.target - 1) / p.target, static_cast<int64_t>(kSplitWarps)),
-                                  static_cast<int64_t>(p.chunk)));
+    // Runs of `chunk` tiles, equal for the whole batch, about p.share of them and at most p.fit
+    auto clamp_chunk = [&](int64_t n) {
+      return static_cast<int>(min(max(n, static_cast<int64_t>(kSplitWarps)), static_cast<int64_t>(p.chunk)));
     };
     if (p.c.batch == 1 || p.plan == nullptr) {       // one sequence, or none is split
       b = p.plan == nullptr ? slot : 0;
       const int tiles = split_tiles(p, b, KT, t0);
-      chunk = p.plan == nullptr ? max(tiles, 1) : chunk_of(tiles);
+      chunk = p.plan == nullptr ? max(tiles, 1) : clamp_chunk((tiles + p.share - 1) / p.share);
       splits = max(1, (tiles + chunk - 1) / chunk);
       first_slot = b;
       if (slot >= first_slot + splits) return;
-    } else {                                         // every block scans the lengths
-      __shared__ int s_warp[kSplitWarps];
-      const int per = (p.c.batch + kThreads - 1) / kThreads;
-      const int b0 = tid * per, b1 = min(b0 + per, p.c.batch);
-      int sum = 0, base;
-      for (int i = b0; i < b1; ++i) sum += split_tiles(p, i, KT, base);
+    } else {                                         // every warp scans the lengths
+      int base, sum = 0, longest = 0;
+      const bool wide = p.c.batch > 32;              // more than a warp's: the block's warps share them
+      for (int i = wide ? tid : lane; i < p.c.batch; i += wide ? kThreads : 32) {
+        const int tiles = split_tiles(p, i, KT, base);
+        sum += tiles;
+        longest = max(longest, tiles);
+      }
       sum = __reduce_add_sync(0xffffffffu, sum);
-      if (lane == 0) s_warp[warp] = sum;
-      if (tid == 0) s_red[0] = -1;
-      __syncthreads();
-      sum = 0;
+      longest = __reduce_max_sync(0xffffffffu, longest);
+      if (wide) {
+        __shared__ int2 s_sum[kSplitWarps];
+        if (lane == 0) s_sum[warp] = make_int2(sum, longest);
+        __syncthreads();
+        sum = longest = 0;
 #pragma unroll
-      for (int w = 0; w < kSplitWarps; ++w) sum += s_warp[w];
-      chunk = chunk_of(sum);
-      int mine = 0;
-      for (int i = b0; i < b1; ++i) mine += max(1, (split_tiles(p, i, KT, base) + chunk - 1) / chunk);
-      int incl = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += up;
+        for (int w = 0; w < kSplitWarps; ++w) sum += s_sum[w].x, longest = max(longest, s_sum[w].y);
       }
-      __syncthreads();
-      if (lane == 31) s_warp[warp] = incl;
-      __syncthreads();
-      int before = incl - mine;
-      for (int w = 0; w < warp; ++w) before += s_warp[w];
-      for (int i = b0; i < b1; ++i) {
-        const int n = max(1, (split_tiles(p, i, KT, t0) + chunk - 1) / chunk);
-        if (slot >= before && slot < before + n) {
-          s_red[0] = i;
-          s_red[1] = before;
-          s_red[2] = n;
+      chunk = clamp_chunk((sum + p.share - 1) / p.share);
+      if (p.fit < p.c.batch + p.share) {
+        // Sequences end inside runs, so more come out than that.  A length that does for p.fit in any case, and the
+        // eighths down to the one above; each warp counts the runs of two of them.
+        __shared__ int s_runs[2 * kSplitWarps];
+        const int lo = chunk;
+        const int hi = p.fit > p.c.batch ? clamp_chunk((sum + p.fit - p.c.batch - 1) / (p.fit - p.c.batch)) : p.chunk;
+        auto eighth = [&](int i) { return lo + (hi - lo) * i / (2 * kSplitWarps); };
+        const int c0 = eighth(2 * warp), c1 = eighth(2 * warp + 1);
+        int runs0 = 0, runs1 = 0;
+        for (int i = lane; i < p.c.batch; i += 32) {
+          const int tiles = split_tiles(p, i, KT, base);
+          runs0 += max(1, (tiles + c0 - 1) / c0);
+          runs1 += max(1, (tiles + c1 - 1) / c1);
         }
-        before += n;
+        runs0 = __reduce_add_sync(0xffffffffu, runs0);
+        runs1 = __reduce_add_sync(0xffffffffu, runs1);
+        if (lane == 0) s_runs[2 * warp] = runs0, s_runs[2 * warp + 1] = runs1;
+        __syncthreads();
+        chunk = hi;
+#pragma unroll
+        for (int i = 2 * kSplitWarps - 1; i >= 0; --i)
+          if (s_runs[i] <= p.fit) chunk = eighth(i);
       }
-      __syncthreads();
-      b = s_red[0];
-      if (b < 0) return;
-      first_slot = s_red[1];
-      splits = s_red[2];
+      if (longest <= chunk) {
+        if (slot >= p.c.batch) return;
+        b = first_slot = slot;
+        splits = 1;
+      } else {
+        int mine = 0;                                // a lane has every 32nd sequence; runs go by lane, then sequence
+        for (int i = lane; i < p.c.batch; i += 32) mine += max(1, (split_tiles(p, i, KT, base) + chunk - 1) / chunk);
+        int before = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane >= o) before += up;
+        }
+        before -= mine;
+        b = -1, first_slot = splits = 0;
+        for (int i = lane; i < p.c.batch; i += 32) {
+          const int n = max(1, (split_tiles(p, i, KT, base) + chunk - 1) / chunk);
+          if (slot >= before && slot < before + n) b = i, first_slot = before, splits = n;
+          before += n;
+        }
+        const unsigned found = __ballot_sync(0xffffffffu, b >= 0);
+        if (!found) return;
+        const int from = __ffs(found) - 1;
+        b = __shfl_sync(0xffffffffu, b, from);
+        first_slot = __shfl_sync(0xffffffffu, first_slot, from);
+        splits = __shfl_sync(0xffffffffu, splits, from);
+      }
     }
     split = slot - first_slot;
     const int tiles = split_tiles(p, b, KT, t0);
@@ -527,7 +553,8 @@ template <typename T, int D, KvParts kParts>
 __global__ void __launch_bounds__(128) attention_kv_join_kernel(const KvAttnParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hk = blockIdx.y, b = blockIdx.z;
-  const int full = blockIdx.x * 4 + warp;          // row of the (sequence, kv head): token * group + head
+  const int per = p.join_warps, sub = warp % per;   // warps a row has
+  const int full = blockIdx.x * (4 / per) + warp / per;   // row of the (sequence, kv head): token * group + head
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (full >= p.group * p.tokens) return;
   const int t = full / p.group, g = full % p.group, h = hk * p.group + g;
@@ -559,15 +586,16 @@ __global__ void __launch_bounds__(128) attention_kv_join_kernel(const KvAttnPara
   m = warp_max(m);
   const float ref = m == -INFINITY ? 0.0f : m;
   float l = 0.0f, o[D / 32] = {};
-  for (int s0 = 0; s0 < n; s0 += 32) {
+  const int share = (n + per - 1) / per, mine1 = min(n, sub * share + share);
+  for (int s0 = sub * share; s0 < mine1; s0 += 32) {
     float f = 0.0f;
-    if (s0 + lane < n) {
+    if (s0 + lane < mine1) {
       const float2 ml = *reinterpret_cast<const float2*>(src + (s0 + lane) * step + D);
       f = ex2_approx(ml.x - ref);
       l = __fmaf_rn(ml.y, f, l);
     }
-    const int end = min(32, n - s0);
-#pragma unroll 4
+    const int end = min(32, mine1 - s0);
+#pragma unroll 8
     for (int s = 0; s < end; ++s) {
       const float fs = __shfl_sync(0xffffffffu, f, s);
       const float* v = src + (s0 + s) * step + lane * (D / 32);
@@ -580,6 +608,23 @@ __global__ void __launch_bounds__(128) attention_kv_join_kernel(const KvAttnPara
     }
   }
   l = warp_sum(l);
+  if (per > 1) {            // four warps, one row a block
+    __shared__ float s_part[4][D + 1];
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) s_part[warp][lane * (D / 32) + k] = o[k];
+    if (lane == 0) s_part[warp][D] = l;
+    __syncthreads();
+    if (warp > 0) return;
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) l += s_part[w][D];
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) {
+      o[k] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) o[k] += s_part[w][lane * (D / 32) + k];
+    }
+  }
   const float f = l == 0.0f ? 0.0f : __frcp_rn(l);
   T* out = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1] + t * p.os[2] + lane * (D / 32);
 #pragma unroll

@@ -592,3 +592,25 @@ def test_long_single_streams(cuda_lib):
         got = K.attention_kv_i8(q, cache, table[pick].contiguous(), _i32(n), 0.09)
         out, _, bound = _attend_all(ref, [rows[i] for i in pick], q, n, [t] * len(pick), 0.09, 128)
         R.check(got, out, bound, torch.bfloat16)
+
+
+@pytest.mark.parametrize("heads,group,dim,lens", [
+    (8, 1, 64, [4000, 17, 2900, 0, 3333, 1, 640, 3969, 64, 2500]),            # cut to fit one wave of blocks
+    (8, 20, 64, [3100, 900, 2047, 33]),                                       # two row tiles
+    (8, 2, 128, [1800, 5, 2100, 700] * 4),
+    (8, 2, 64, [5000, 3000] + [(37 * i) % 200 for i in range(43)]),           # more than a warp's, three waves
+    (8, 1, 64, [2500] + [(53 * i) % 150 for i in range(62)] + [1900]),        # more rows than blocks
+    (8, 1, 64, [(29 * i) % 120 for i in range(127)] + [4100, 0, 2000]),       # more than twice as many
+    (8, 1, 64, [(29 * i) % 120 for i in range(130)]),                         # and none long enough to cut
+])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_attention_uneven_batches(cuda_lib, heads, group, dim, lens, dtype):
+    """Sequences of very different lengths, cut into runs that fit the device."""
+    from h3vae_b200 import kernels as K
+    rng = np.random.default_rng(len(lens))
+    ref, rows, table = _filled(rng, lens, heads, dim, 64)
+    cache = _cache(ref)
+    q = torch.from_numpy(rng.standard_normal((len(lens), heads * group, 1, dim)) * 2).to(TYPES[dtype]).cuda()
+    got = K.attention_kv_i8(q, cache, _wide(table, 2000), _i32(lens), dim ** -0.5)
+    out, _, bound = _attend_all(ref, rows, q, lens, [1] * len(lens), dim ** -0.5, 64)
+    R.check(got, out, bound, TYPES[dtype])
