@@ -213,7 +213,8 @@ extern "C" int h3b_attention_kv_i8(const void* q, const int64_t* q_strides, cons
   if (tokens == 0) return H3B_OK;
   const KvPlan k = kv_plan(batch, q_heads, cache->kv_heads, tokens, cache->head_dim, table_width, cache->page_size,
                            selected ? n_selected : 0);
-  if (!workspace || !h3b_host::aligned16(workspace) || workspace_bytes < 16 + k.plan_bytes + k.part_bytes)
+  const size_t need = k.plan_bytes + k.part_bytes;
+  if (need && (!workspace || !h3b_host::aligned16(workspace) || workspace_bytes < 16 + need))
     return h3b_host::set_error(H3B_EINVAL, "%s: workspace missing, misaligned or too small", name);
   p.q = q;
   p.out = out;

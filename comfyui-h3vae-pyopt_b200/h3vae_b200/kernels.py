@@ -869,7 +869,7 @@ def attention_kv_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: t
     dev, dim = cache.device, cache.head_dim
     if out is None:
         strides = (tokens * heads * dim, dim, heads * dim, 1)
-        out = torch.empty_strided((batch, heads, tokens, dim), strides, device=dev, dtype=q.dtype)
+        out = q.new_empty_strided((batch, heads, tokens, dim), strides)
         out_strides = _pack3(*strides[:3])
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise ValueError("out must have q's shape and dtype")
@@ -888,11 +888,11 @@ def attention_kv_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: t
         lib = _lib.load()
         ws_bytes = _kv_workspace_bytes("h3b_attention_kv_i8", batch, heads, cache.kv_heads, tokens, dim, width,
                                        cache.page_size, n_sel)
-        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+        ws = cache.k.new_empty(ws_bytes) if ws_bytes > 16 else None      # 16: the call needs none
         _lib.check(lib.h3b_attention_kv_i8(
             q.data_ptr(), q_strides, cache.struct, table, batch, width, _kv_index(lengths, "lengths", (batch,), dev),
             _kv_index(counts, "counts", (batch,), dev), heads, tokens, float(scale), 1 if causal else 0, window,
-            _ptr(selected), n_sel, _KV_TYPES[q.dtype], out.data_ptr(), out_strides, _ptr(lse), ws.data_ptr(),
+            _ptr(selected), n_sel, _KV_TYPES[q.dtype], out.data_ptr(), out_strides, _ptr(lse), _ptr(ws),
             ws_bytes, _kv_stream(dev)))
         _count(1)
     return (out, lse) if return_lse else out
@@ -908,11 +908,11 @@ def kv_select_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torc
     dev = cache.device
     if pages < 1 or lengths is None:
         raise ValueError("pages must be at least 1 and lengths int32 [batch]")
-    selected = torch.empty((batch, cache.kv_heads, tokens, pages), device=dev, dtype=_I32)
+    selected = page_table.new_empty((batch, cache.kv_heads, tokens, pages))
     if tokens:
         lib = _lib.load()
         ws_bytes = _kv_workspace_bytes("h3b_kv_select_i8", batch, cache.kv_heads, tokens, width)
-        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+        ws = cache.k.new_empty(ws_bytes)
         _lib.check(lib.h3b_kv_select_i8(
             q.data_ptr(), q_strides, cache.struct, table, batch, width, _kv_index(lengths, "lengths", (batch,), dev),
             _kv_index(counts, "counts", (batch,), dev), heads, tokens, pages, _KV_TYPES[q.dtype], selected.data_ptr(),
