@@ -917,5 +917,5 @@ def kv_select_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torc
             q.data_ptr(), q_strides, cache.struct, table, batch, width, _kv_index(lengths, "lengths", (batch,), dev),
             _kv_index(counts, "counts", (batch,), dev), heads, tokens, pages, _KV_TYPES[q.dtype], selected.data_ptr(),
             ws.data_ptr(), ws_bytes, _kv_stream(dev)))
-        _count(2)
+        _count(1)
     return selected

@@ -614,3 +614,23 @@ def test_attention_uneven_batches(cuda_lib, heads, group, dim, lens, dtype):
     got = K.attention_kv_i8(q, cache, _wide(table, 2000), _i32(lens), dim ** -0.5)
     out, _, bound = _attend_all(ref, rows, q, lens, [1] * len(lens), dim ** -0.5, 64)
     R.check(got, out, bound, TYPES[dtype])
+
+
+@pytest.mark.parametrize("heads,group,t,width,n", [(2, 3, 1, 60, 5), (1, 1, 3, 900, 40), (2, 2, 8, 1600, 33), (3, 8, 8, 2100, 64),
+                                                   (1, 1, 1, 4096, 9), (16, 1, 8, 1030, 16), (1, 9, 8, 1600, 12), (2, 1, 9, 1600, 7)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_select_wide_tables(cuda_lib, heads, group, t, width, n, dim):
+    """One launch or two, by tokens and the table's width: the same choice as with a table no wider than needed."""
+    from h3vae_b200 import kernels as K
+    rng = np.random.default_rng(width + n)
+    lens = [1000, 0, 16 * min(width, 1200) - 3]
+    ref, rows, table = _filled(rng, lens, heads, dim, 16)
+    cache = _cache(ref)
+    q = torch.from_numpy(rng.standard_normal((3, heads * group, t, dim))).half().cuda()
+    wide = torch.nn.functional.pad(table, (0, max(0, width - table.shape[1])), value=-1).contiguous()
+    got = K.kv_select_i8(q, cache, wide, _i32(lens), n)
+    for other in (table, _wide(table, 5000)):
+        assert torch.equal(got, K.kv_select_i8(q, cache, other, _i32(lens), n))
+    counts = [t, t, max(t - 1, 0)]
+    got = K.kv_select_i8(q, cache, wide, _i32(lens), n, counts=_i32(counts))
+    assert torch.equal(got, K.kv_select_i8(q, cache, _wide(table, 5000), _i32(lens), n, counts=_i32(counts)))
