@@ -503,26 +503,39 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
       float back;
       {
         const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1] + t * p.qs[2];
-        float top = 0.0f;
-        if (sizeof(T) == 2 && real) {
-#pragma unroll 1
-          for (int i = 0; i < D / 8; ++i) {
-            float x[8];
-            load8(q + 8 * i, p.vec_q, x);
+        uint4 raw[D / 8];      // the whole row in flight: a load at a time cost the CTA 7 us before its first product
+        if (real && p.vec_q) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+          for (int i = 0; i < D / 8; ++i) raw[i] = *reinterpret_cast<const uint4*>(q + 8 * i);
+        } else {
+          const unsigned short* bits = reinterpret_cast<const unsigned short*>(q);
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = real ? bits[8 * i + 2 * e] | static_cast<uint32_t>(bits[8 * i + 2 * e + 1]) << 16 : 0u;
+            raw[i] = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
+        auto element = [&](int i) {
+          const uint4& v = raw[i >> 3];
+          const uint32_t w = (i & 7) < 2 ? v.x : (i & 7) < 4 ? v.y : (i & 7) < 6 ? v.z : v.w;
+          const unsigned short half = static_cast<unsigned short>(i & 1 ? w >> 16 : w);
+          return to_f32(reinterpret_cast<const T&>(half));
+        };
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D; ++i) top = fmaxf(top, fabsf(element(i)));
         // a negative scale turns the row, so that larger products are larger scores
         const float f = row_scaling(T(), top, back) * (p.scale_log2 < 0.0f ? -1.0f : 1.0f);
         const uint32_t dst = smem_u32(sq + tile * L::kTile) + row * 128;
-#pragma unroll 1
+#pragma unroll
         for (int i = 0; i < D / 8; ++i) {
-          float x[8] = {};
-          if (real) load8(q + 8 * i, p.vec_q, x);
           uint32_t w[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = h2_bits(__floats2half2_rn(x[2 * e] * f, x[2 * e + 1] * f));
+          for (int e = 0; e < 4; ++e)
+            w[e] = h2_bits(__floats2half2_rn(element(8 * i + 2 * e) * f, element(8 * i + 2 * e + 1) * f));
           st_shared_v4(dst + (i >> 3) * 16384 + (((i & 7) ^ (row & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
         }
         fence_proxy_async_smem();
