@@ -256,6 +256,36 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
     blk0 += from;
   }
 
+  // The converters' first lookups run under the set-up below: the pages of the units that a warp copies first, and
+  // pages and scales of the first two batches of blocks (see there).
+  const int units = 4 * n_blocks;
+  const int seg_keys = min(p.c.page, kKtUnit), segs = kKtUnit / seg_keys;
+  int look_page = -1, ahead_page[L::kStages];
+  float look_k = 0.0f, look_v = 0.0f;
+  auto look_pages = [&](int m) {
+    const int key = (blk0 + m * kKtBatch) * kKtKeys + 16 * lane;
+    look_page = -1;
+    if (16 * m < units && key < len) look_page = kv_page(p.c, b, key >> p.c.page_shift);
+  };
+  auto look_scales = [&]() {
+    if (look_page >= 0) {
+      const int64_t ph = static_cast<int64_t>(look_page) * p.c.heads + hk;
+      look_k = p.c.scale[0][ph];
+      look_v = p.c.scale[1][ph];
+    }
+  };
+  if (warp < kKtConvWarps) {
+#pragma unroll
+    for (int st = 0; st < L::kStages; ++st) {
+      const int g = warp + st * kKtConvWarps, key = (blk0 + (g >> 2)) * kKtKeys + (g & 1) * kKtUnit + lane * seg_keys;
+      ahead_page[st] = lane < segs && g < units && key < len ? kv_page(p.c, b, key >> p.c.page_shift) : -1;
+    }
+    if (warp < 2) {
+      look_pages(warp);
+      look_scales();
+    }
+  }
+
   if (threadIdx.x == 0) {
     mbar_init(q_full, 32 * 4 * tiles);
     for (int s = 0; s < NS; ++s) {
@@ -292,28 +322,12 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
     constexpr int kVecs = kKtUnit * kPerKey / 32;          // of a unit, a lane
     constexpr int kKeyStep = 32 / kPerKey;
     const int key_in = lane / kPerKey, col = lane % kPerKey;
-    const int units = 4 * n_blocks;
-    const int seg_keys = min(p.c.page, kKtUnit), segs = kKtUnit / seg_keys;
     const uint32_t seg_bytes = seg_keys * D;
     const uint32_t stage0 = smem_u32(staged + warp * L::kStages * L::kUnit);
     uint64_t* full = staged_full + warp * L::kStages;
     // Pages and scales are looked up for four blocks at a time, a lane for each 16 keys, two batches ahead, and in
     // three steps a unit apart, so that no load is waited for.  Batch m is the affair of the warp that has the
     // first unit of batch m - 2.  (Each warp looking up its own units' took 1400 cycles a unit.)
-    int look_page = -1;
-    float look_k = 0.0f, look_v = 0.0f;
-    auto look_pages = [&](int m) {
-      const int key = (blk0 + m * kKtBatch) * kKtKeys + 16 * lane;
-      look_page = -1;
-      if (16 * m < units && key < len) look_page = kv_page(p.c, b, key >> p.c.page_shift);
-    };
-    auto look_scales = [&]() {
-      if (look_page >= 0) {
-        const int64_t ph = static_cast<int64_t>(look_page) * p.c.heads + hk;
-        look_k = p.c.scale[0][ph];
-        look_v = p.c.scale[1][ph];
-      }
-    };
     auto write_meta = [&](int m) {
       float4 f = make_float4(1.0f, -INFINITY, 0.0f, __int_as_float(-1));       // no page: weight 0
       if (look_page >= 0) {   // a scale of zero: a page never written holds zeros
@@ -338,8 +352,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
     auto page_of = [&](int g, int in) {
       return __float_as_int(s_meta[((g >> 2) % kKtMeta) * 8 + ((g & 1) * kKtUnit + in) / 16].w);
     };
-    auto issue = [&](int g, int stage) {   // lane j copies segment j
-      const int page = lane < segs ? page_of(g, lane * seg_keys) : -1;
+    auto issue = [&](int g, int stage, int page) {   // lane j copies segment j
       const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
       if (lane == 0) mbar_arrive_expect_tx(&full[stage], seg_bytes * __popc(there));
       __syncwarp();
@@ -351,18 +364,14 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
                   smem_u32(&full[stage]));
       }
     };
-    if (warp < 2 && 16 * warp < units) {
-      look_pages(warp);
-      look_scales();
-      write_meta(warp);
-    }
     int stage = 0;
     uint32_t phase = 0;
-    bool ok = units == 0 || know(0);
     int issued = 0;
-#pragma unroll 1
+#pragma unroll
     for (int st = 0; st < L::kStages; ++st)
-      if (ok && warp + st * kKtConvWarps < units) issue(warp + st * kKtConvWarps, st), ++issued;
+      if (warp + st * kKtConvWarps < units) issue(warp + st * kKtConvWarps, st, ahead_page[st]), ++issued;
+    if (warp < 2 && 16 * warp < units) write_meta(warp);
+    bool ok = units == 0 || know(0);
     int g = warp;
     for (; ok && g < units; g += kKtConvWarps) {
       const bool is_v = (g >> 1) & 1;
@@ -428,7 +437,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
       if (lane == 0) mbar_arrive(&slot_full[s]);
       if (after < units) {
         ok = know(after);
-        if (ok) issue(after, stage);
+        if (ok) issue(after, stage, lane < segs ? page_of(after, lane * seg_keys) : -1);
       }
       if (++stage == L::kStages) stage = 0, phase ^= 1;
     }
