@@ -28,11 +28,14 @@
 // clock: 45 % at dim 64), but the chain of a row tile -- products, wait, weights (2000
 // to 2200 cycles a block), wait, products -- which two row tiles only half cover, and
 // at dim 128 the converters beside it.  1024 tokens over 5120 keys, 2 x
-// 16 heads of dim 64: 85 us = 505 TFLOP/s; a causal prompt of 8101 tokens, 2 x 32
-// heads over 8 of dim 128: 1.27 ms = 850 TFLOP/s.  Measured and left: 64-key steps with
-// two buffers of products (99 us, 1.45 ms: twice the waits of the issuing warp), 16
+// 16 heads of dim 64: 84 us = 510 TFLOP/s; a causal prompt of 8101 tokens, 2 x 32
+// heads over 8 of dim 128: 1.16 ms = 927 TFLOP/s.  A call over 256 keys takes
+// 12 us at dim 64 and 17 at dim 128, every further 128 keys 2.0 and 2.3.  Measured and
+// left, against 85 us and 1.27 ms: 64-key steps with two buffers of products (99 us, 1.45 ms: twice the waits of the issuing warp), 16
 // warps with an issuer per row tile and six converters (91 us, 1.52 ms: 128 registers
 // a thread), all 128 products of a row in registers (109 us, 1.65 ms).
+#include <type_traits>
+
 #include "attention_kv.cuh"
 
 namespace h3b {
@@ -205,6 +208,117 @@ __device__ __forceinline__ float weights(uint32_t taddr, uint32_t meta, float ba
     sum = __fmaf_rn(a0 + a1, f.z, sum);
   }
   return sum;
+}
+
+// A warp's 32 rows move between global and shared memory with a row over D / 8
+// lanes (a row a lane touches 32 lines an instruction: 4000 cycles each way at dim
+// 128), 16-byte chunks in the tile's swizzle.  The way out is out of line for the
+// registers of the softmax loop, the way in is not (256 rows of fp16, dim 128, over 4096
+// keys: 87 us, both inside 91; a bf16 prompt: 1160 us, both out of line 1230).
+__device__ __forceinline__ uint32_t chunk_at(uint32_t rows_at, int row, int chunk) {
+  return rows_at + row * 128 + (chunk >> 3) * 16384 + (((chunk & 7) ^ (row & 7)) << 4);
+}
+
+// Q: `mine` is this lane's row (null: zeros); returns what its products are scaled back by.
+template <typename T, int D>
+__device__ __forceinline__ float load_rows(const T* mine, bool vec, float sign, uint32_t rows_at) {
+  constexpr int kLanes = D / 8, kStepRows = 32 / kLanes;
+  const int lane = threadIdx.x & 31, in_row = lane / kLanes, chunk = lane % kLanes;
+  uint4 raw[D / 8];      // all in flight
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) {
+    const T* q = reinterpret_cast<const T*>(
+        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), i * kStepRows + in_row));
+    raw[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (q && vec) {
+      raw[i] = *reinterpret_cast<const uint4*>(q + 8 * chunk);
+    } else if (q) {
+      const unsigned short* bits = reinterpret_cast<const unsigned short*>(q + 8 * chunk);
+      raw[i] = make_uint4(bits[0] | static_cast<uint32_t>(bits[1]) << 16, bits[2] | static_cast<uint32_t>(bits[3]) << 16,
+                          bits[4] | static_cast<uint32_t>(bits[5]) << 16, bits[6] | static_cast<uint32_t>(bits[7]) << 16);
+    }
+  }
+  float back = 1.0f;
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) {
+    const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+    float x[8], top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned short half = static_cast<unsigned short>(words[e >> 1] >> (16 * (e & 1)));
+      x[e] = to_f32(reinterpret_cast<const T&>(half));
+      top = fmaxf(top, fabsf(x[e]));
+    }
+    float row_back, f;
+    if (std::is_same<T, __half>::value) {
+      f = sign * row_scaling(T(), top, row_back);
+    } else {
+#pragma unroll
+      for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      f = sign * row_scaling(T(), top, row_back);
+      row_back = __shfl_sync(0xffffffffu, row_back, (lane % kStepRows) * kLanes);
+      if (lane / kStepRows == i) back = row_back;
+    }
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = h2_bits(__floats2half2_rn(x[2 * e] * f, x[2 * e + 1] * f));
+    st_shared_v4(chunk_at(rows_at, i * kStepRows + in_row, chunk), make_uint4(w[0], w[1], w[2], w[3]));
+  }
+  return back;
+}
+
+// 32 columns of a row's O out of TMEM, zeros where there is none.
+__device__ __forceinline__ void load_o(uint32_t taddr, bool have, uint32_t (&r)[32]) {
+  if (have) {
+    tmem_ld32(taddr, r);
+    tmem_ld_wait();
+  } else {
+#pragma unroll
+    for (int d = 0; d < 32; ++d) r[d] = 0u;
+  }
+}
+
+// O: to `out` times inv, or as it is to `part`, D * 2 bytes of a row at a time (null rows are not written).
+template <typename T, int D>
+__device__ __noinline__ void store_rows(uint32_t t_o, bool have, float inv, T* out, float* part, bool parts, uint32_t rows_at) {
+  constexpr int kLanes = D / 8, kStepRows = 32 / kLanes;
+  const int lane = threadIdx.x & 31, in_row = lane / kLanes, chunk = lane % kLanes;
+  const unsigned long long mine =
+      parts ? reinterpret_cast<unsigned long long>(part) : reinterpret_cast<unsigned long long>(out);
+#pragma unroll 1
+  for (int round = 0; round < (parts ? 2 : 1); ++round) {
+    uint32_t r[32];
+    if (parts) {
+#pragma unroll 1
+      for (int c = 0; c < D / 64; ++c) {
+        load_o(t_o + round * (D / 2) + c * 32, have, r);
+#pragma unroll
+        for (int v = 0; v < 8; ++v)
+          st_shared_v4(chunk_at(rows_at, lane, c * 8 + v), make_uint4(r[4 * v], r[4 * v + 1], r[4 * v + 2], r[4 * v + 3]));
+      }
+    } else {
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        load_o(t_o + c * 32, have, r);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          __align__(16) T y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) from_f32(__uint_as_float(r[8 * v + e]) * inv, y[e]);
+          st_shared_v4(chunk_at(rows_at, lane, c * 4 + v), *reinterpret_cast<const uint4*>(y));
+        }
+      }
+    }
+    __syncwarp();
+#pragma unroll 4
+    for (int i = 0; i < D / 8; ++i) {
+      const int row = i * kStepRows + in_row;
+      const unsigned long long to = __shfl_sync(0xffffffffu, mine, row);
+      const uint4 v = ld_shared_v4(chunk_at(rows_at, row, chunk));
+      if (to) *reinterpret_cast<uint4*>(to + round * (D * 2) + chunk * 16) = v;
+    }
+    __syncwarp();
+  }
 }
 
 template <typename T, int D>
@@ -508,45 +622,13 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
       int first = 0, last = 0x7fffffff;                      // rows past the end never force masking
       if (real) kv_range(p, len, n_tok, t, first, last);
       const int first_max = __reduce_max_sync(0xffffffffu, first), last_min = __reduce_min_sync(0xffffffffu, last);
-      // Q row to shared memory
+      // Q rows to shared memory
+      const uint32_t rows_at = smem_u32(sq + tile * L::kTile) + quad * 32 * 128;      // this warp's
       float back;
       {
-        const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1] + t * p.qs[2];
-        uint4 raw[D / 8];      // the whole row in flight: a load at a time cost the CTA 7 us before its first product
-        if (real && p.vec_q) {
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i) raw[i] = *reinterpret_cast<const uint4*>(q + 8 * i);
-        } else {
-          const unsigned short* bits = reinterpret_cast<const unsigned short*>(q);
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = real ? bits[8 * i + 2 * e] | static_cast<uint32_t>(bits[8 * i + 2 * e + 1]) << 16 : 0u;
-            raw[i] = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-        auto element = [&](int i) {
-          const uint4& v = raw[i >> 3];
-          const uint32_t w = (i & 7) < 2 ? v.x : (i & 7) < 4 ? v.y : (i & 7) < 6 ? v.z : v.w;
-          const unsigned short half = static_cast<unsigned short>(i & 1 ? w >> 16 : w);
-          return to_f32(reinterpret_cast<const T&>(half));
-        };
-        float top = 0.0f;
-#pragma unroll
-        for (int i = 0; i < D; ++i) top = fmaxf(top, fabsf(element(i)));
-        // a negative scale turns the row, so that larger products are larger scores
-        const float f = row_scaling(T(), top, back) * (p.scale_log2 < 0.0f ? -1.0f : 1.0f);
-        const uint32_t dst = smem_u32(sq + tile * L::kTile) + row * 128;
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = h2_bits(__floats2half2_rn(element(8 * i + 2 * e) * f, element(8 * i + 2 * e + 1) * f));
-          st_shared_v4(dst + (i >> 3) * 16384 + (((i & 7) ^ (row & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
-        }
+        const T* mine = real ? static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1] + t * p.qs[2] : nullptr;
+        // a negative scale turns the rows, so that larger products are larger scores
+        back = load_rows<T, D>(mine, p.vec_q, p.scale_log2 < 0.0f ? -1.0f : 1.0f, rows_at);
         fence_proxy_async_smem();
         mbar_arrive(q_full);
       }
@@ -603,37 +685,21 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
       const bool have = ok && n_blocks > 0;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       if (have) tc_fence_after();
+      T* out = real ? static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1] + t * p.os[2] : nullptr;
+      float* part = nullptr;
+      if (real && p.part)
+        part = p.part + ((((static_cast<int64_t>(split) * p.c.batch + b) * p.c.heads + hk) * g_rows) + full) * (D + 4);
+      if (p.part || p.vec_out) {
+        store_rows<T, D>(t_o, have, inv, out, part, p.part != nullptr, rows_at);   // over Q: every product with it is done
+        if (part) *reinterpret_cast<float2*>(part + D) = make_float2(m, l);
+      } else {
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t r[32];
-        if (have) {
-          tmem_ld32(t_o + c * 32, r);
-          tmem_ld_wait();
-        } else {
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t r[32];
+          load_o(t_o + c * 32, have, r);
+          if (!real) continue;
 #pragma unroll
-          for (int d = 0; d < 32; ++d) r[d] = 0u;
-        }
-        if (!real) continue;
-        if (p.part) {
-          float* dst = p.part + ((((static_cast<int64_t>(split) * p.c.batch + b) * p.c.heads + hk) * g_rows) + full) * (D + 4);
-#pragma unroll
-          for (int d = 0; d < 32; d += 4)
-            *reinterpret_cast<uint4*>(dst + c * 32 + d) = make_uint4(r[d], r[d + 1], r[d + 2], r[d + 3]);
-          if (c == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m, l);
-        } else {
-          T* dst = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1] + t * p.os[2] + c * 32;
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            __align__(16) T y[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) from_f32(__uint_as_float(r[8 * v + e]) * inv, y[e]);
-            if (p.vec_out) {
-              *reinterpret_cast<uint4*>(dst + 8 * v) = *reinterpret_cast<const uint4*>(y);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) dst[8 * v + e] = y[e];
-            }
-          }
+          for (int d = 0; d < 32; ++d) from_f32(__uint_as_float(r[d]) * inv, out[c * 32 + d]);
         }
       }
       if (real && p.lse && !p.part)
