@@ -11,10 +11,10 @@ namespace {
 // The tensor-core tiles are taken above kTileRows rows of a (sequence, kv head)
 // if the 16-row tiles of the other kernel would read more than kTileBytes of
 // codes.  Measured, tiles against 16-row tiles, us: 16 heads over 5120 keys, dim 64:
-// 33 rows 19.5 / 14.7, 64 rows 19.9 / 26.4; 8 x 8 heads over 8192 keys, dim 128: 20
-// rows 78 / 77, 36 rows 79 / 99, 128 rows 83 / 225; 32 x 16 heads over 2000 keys: 40
-// rows 130 / 97, 70 rows 131 / 151; 8 heads over 1000 keys, dim 128: 128 rows (16 MB)
-// 22 / 12, 256 rows (33 MB) 28 / 28.
+// 33 rows 20 / 16, 64 rows 20 / 19; 8 x 8 heads over 8192 keys, dim 128, fp16 and
+// bf16: 17 rows 80 / 81 and 72, 33 rows 80 / 112 and 99, 64 rows 81 / 144 and 128; 32 x
+// 16 heads over 2000 keys: 40 rows 127 / 103, 70 rows 128 / 163; 2 x 16 heads over 1024 keys:
+// 64 rows (17 MB) 17 / 12, 128 rows (34 MB) 18 / 33.
 constexpr int64_t kTileRows = 48;
 constexpr int64_t kTileBytes = int64_t(24) << 20;
 

@@ -32,7 +32,7 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
 // bytes once and is bound by HBM when it is long and by latency (table, scale
 // and code loads in a row, then the join) when it is short.  One token each over
 // 16 x 6553..32768 keys, 8 heads of dim 128, 32 query heads: 690 MB in 129 us =
-// 5.3 TB/s, with the issue slots 56 % and the tensor pipe 32 % in use; 12 warps an
+// 5.3 TB/s, with the issue slots 52 % and the tensor pipe 34 % in use; 12 warps an
 // SM hide each other's latency.  Before runs were fitted to waves, at 141 us: 8 warps
 // 154 us, tiles of half the size 165 us, of twice the size 178 us.  One token over 1797 keys of 16 heads: 6.5 us.
 constexpr int kSplitWarps = 4;

@@ -24,16 +24,16 @@
 // the block redone and O rescaled in TMEM.  Blocks that no row of the CTA sees are
 // not visited, and only blocks on an edge of a row's range mask keys.
 //
-// What bounds it: not the tensor pipe (22 % active) nor the SFU (16 exponentials a
-// clock: 45 % at dim 64), but the chain of a row tile -- products, wait, weights (2000
-// to 2200 cycles a block), wait, products -- which two row tiles only half cover, and
-// at dim 128 the converters beside it.  1024 tokens over 5120 keys, 2 x
-// 16 heads of dim 64: 84 us = 510 TFLOP/s; a causal prompt of 8101 tokens, 2 x 32
-// heads over 8 of dim 128: 1.16 ms = 927 TFLOP/s.  A call over 256 keys takes
-// 12 us at dim 64 and 17 at dim 128, every further 128 keys 2.0 and 2.3.  Measured and
-// left, against 85 us and 1.27 ms: 64-key steps with two buffers of products (99 us, 1.45 ms: twice the waits of the issuing warp), 16
-// warps with an issuer per row tile and six converters (91 us, 1.52 ms: 128 registers
-// a thread), all 128 products of a row in registers (109 us, 1.65 ms).
+// What bounds it: not the tensor pipe (27 % active at dim 64) nor the SFU (16
+// exponentials a clock: 55 %), but the chain of a row tile -- products, wait, weights
+// (2000 to 2200 cycles a block), wait, products -- which two row tiles only half cover,
+// and at dim 128 the converters beside it.  1024 tokens over 5120 keys, 2 x 16 heads of
+// dim 64: 84 us = 510 TFLOP/s; a causal prompt of 8101 tokens, 2 x 32 heads over 8 of dim
+// 128: 1.16 ms = 927 TFLOP/s.  A call over 256 keys takes 12 us at dim 64 and 17 at dim
+// 128, every further 128 keys 2.0 and 2.3.  Measured and left, against 85 us and 1.27 ms:
+// 64-key steps with two buffers of products (99 us, 1.45 ms: twice the waits of the
+// issuing warp), 16 warps with an issuer per row tile and six converters (91 us, 1.52 ms:
+// 128 registers a thread), all 128 products of a row in registers (109 us, 1.65 ms).
 #include <type_traits>
 
 #include "attention_kv.cuh"
