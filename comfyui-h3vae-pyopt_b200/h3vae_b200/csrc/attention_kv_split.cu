@@ -510,7 +510,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_s
   }
   if (p.cluster && splits > 1) {
     // the cluster's blocks join their rows through each other's shared memory, a share of the dims each
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_sync();
     const uint32_t mine = smem_u32(s_c);
     for (int i = split * kThreads + tid; i < rows * (D / 4); i += splits * kThreads) {
       const int row = i / (D / 4), d = (i % (D / 4)) * 4;
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_s
       finish(row, d, acc, mm, ll);
     }
     // no block leaves while another reads its shared memory
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_sync();
   }
 }
 

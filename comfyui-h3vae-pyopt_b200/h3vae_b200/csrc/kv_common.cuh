@@ -37,6 +37,22 @@ __device__ __forceinline__ int kv_page(const KvView& c, int b, int slot) {
   return p;
 }
 
+// The barrier of a cluster's blocks, in its two halves.  The .aligned forms want all
+// lanes of a warp at once, and what comes before (a loop that some lanes leave
+// earlier, a branch) may have split them: the warp is joined first.
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  cluster_arrive();
+  cluster_wait();
+}
+
 template <typename T> struct KvVec8;   // eight elements as 32-bit words
 template <> struct KvVec8<__half> { static constexpr int kWords = 4; };
 template <> struct KvVec8<__nv_bfloat16> { static constexpr int kWords = 4; };

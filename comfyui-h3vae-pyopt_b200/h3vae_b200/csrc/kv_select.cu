@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kThreads) kv_select_kernel(const KvSelectParam
   extern __shared__ __align__(16) uint32_t s_keys[];     // row_keys of this block's token
   const int rank = blockIdx.x, blocks = gridDim.x, head = blockIdx.y, b = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5;
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // waited for below: all blocks run
+  cluster_arrive();   // waited for below: all blocks run
   const int end = kv_last_page(p, b, (p.counts ? min(p.counts[b], p.tokens) : p.tokens) - 1);   // complete pages
   int slot = rank * kThreads + tid, page = slot < end ? kv_page(p.c, b, slot) : -1;
   uint32_t k[D / 2];
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(kThreads) kv_select_kernel(const KvSelectParam
     quantise_row<T, D>(static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1] + t * p.qs[2], s_q[r], &s_s[r]);
   }
   __syncthreads();
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_wait();
   const uint32_t base = smem_u32(s_keys);
   while (slot < end) {
     for (int t = 0; t < p.tokens; ++t) {
@@ -323,8 +323,7 @@ __global__ void __launch_bounds__(kThreads) kv_select_kernel(const KvSelectParam
     page = slot < end ? kv_page(p.c, b, slot) : -1;
     if (page >= 0) load_sums<D>(p, page, head, k, k_scale);
   }
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_sync();
   if (rank >= p.tokens) return;
   const int64_t row = (static_cast<int64_t>(b) * p.c.heads + head) * p.tokens + rank;
   pick_pages<kPer, kThreads, true>(p, s_keys, kv_last_page(p, b, rank), p.selected + row * p.n);

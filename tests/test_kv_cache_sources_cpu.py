@@ -1,0 +1,23 @@
+"""What of the cache kernels is shown by their sources: rules whose breach no run shows reliably."""
+import re
+
+from conftest import PKG_PARENT
+
+CSRC = PKG_PARENT / "h3vae_b200" / "csrc"
+SOURCES = [*sorted(CSRC.glob("kv_*.cu*")), *sorted(CSRC.glob("attention_kv*.cu*"))]
+
+
+def _code(path):
+    return re.sub(r"//[^\n]*", "", path.read_text())
+
+
+def test_aligned_cluster_barriers_join_the_warp_first():
+    """An .aligned barrier needs all lanes of a warp at once: each stands directly behind a __syncwarp()."""
+    found = 0
+    for path in SOURCES:
+        lines = [x.strip() for x in _code(path).splitlines() if x.strip()]
+        for before, line in zip(lines, lines[1:]):
+            if "barrier.cluster" in line and ".aligned" in line:
+                found += 1
+                assert before == "__syncwarp();" and line.count("barrier.cluster") == 1, (path.name, line)
+    assert found
