@@ -202,8 +202,10 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_s
     if (ord >= 0 && static_cast<int64_t>(ord) * p.c.page < len) page = kv_page(p.c, b, ord);
     s_page[i] = page;
   }
-  if (tid < kSplitWarps * kSplitStages) mbar_init(&s_bar[tid], 1);
-  if (tid == 0) fence_barrier_init();
+  if (tid < kSplitWarps * kSplitStages) {
+    mbar_init(&s_bar[tid], 1);
+    fence_barrier_init();     // of this thread's own barrier: a fence orders only what its thread did
+  }
   __syncthreads();
 
   const uint32_t ring = smem_u32(smem) + warp * kSplitStages * kSplitStageBytes;

@@ -21,3 +21,16 @@ def test_aligned_cluster_barriers_join_the_warp_first():
                 found += 1
                 assert before == "__syncwarp();" and line.count("barrier.cluster") == 1, (path.name, line)
     assert found
+
+
+def test_barriers_are_fenced_by_the_thread_that_initialised_them():
+    """A fence after mbarrier.init orders the inits of its own thread: the statement that guards an init guards the
+    fence too, and no second condition stands between them."""
+    found = 0
+    for path in SOURCES:
+        code = _code(path)
+        for match in re.finditer(r"mbar_init\((?:.|\n)*?fence_barrier_init\(\)", code):
+            found += 1
+            assert not re.search(r"\bif\s*\(", match.group(0)), path.name
+        assert code.count("mbar_init(") == 0 or "fence_barrier_init()" in code, path.name
+    assert found
