@@ -697,9 +697,11 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
         for (int c = 0; c < D / 32; ++c) {
           uint32_t r[32];
           load_o(t_o + c * 32, have, r);
-          if (!real) continue;
+          if (real) {
 #pragma unroll
-          for (int d = 0; d < 32; ++d) from_f32(__uint_as_float(r[d]) * inv, out[c * 32 + d]);
+            for (int d = 0; d < 32; ++d) from_f32(__uint_as_float(r[d]) * inv, out[c * 32 + d]);
+          }
+          __syncwarp();     // the next load out of TMEM wants the whole warp
         }
       }
       if (real && p.lse && !p.part)

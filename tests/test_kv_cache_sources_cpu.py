@@ -34,3 +34,12 @@ def test_barriers_are_fenced_by_the_thread_that_initialised_them():
             assert not re.search(r"\bif\s*\(", match.group(0)), path.name
         assert code.count("mbar_init(") == 0 or "fence_barrier_init()" in code, path.name
     assert found
+
+
+def test_warps_stay_whole_around_loads_from_tensor_memory():
+    """tcgen05.ld wants all lanes of a warp: a loop that loads does not let lanes go on to the next round by themselves."""
+    code = _code(CSRC / "attention_kv_tile.cu")
+    for call in re.finditer(r"\b(load_o|tmem_ld32|tmem_ld_wait)\(", code):
+        body = code[call.end():]
+        body = body[: min((body.find(x) for x in ("\n}", "#pragma unroll 1") if x in body), default=len(body))]
+        assert "continue;" not in body, body[:200]
