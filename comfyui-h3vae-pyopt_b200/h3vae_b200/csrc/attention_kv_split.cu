@@ -244,7 +244,9 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_s
       const int64_t ph = static_cast<int64_t>(page) * p.c.heads + hk;
       float vs = p.c.scale[1][ph];
       vs = vs < kKvMinScale ? kKvMinScale : vs;            // a page never written holds zeros; NaN stays
-      f = make_float4(p.c.scale[0][ph] * p.scale_log2, log2f(vs), __frcp_rn(vs), 0.0f);
+      // a NaN scale of V goes with the scores, which are masked, and not with the factor of the sums, which is not:
+      // rows that do not see the page add 0 * (1 / vs)
+      f = make_float4(p.c.scale[0][ph] * p.scale_log2, log2f(vs), isnan(vs) ? 0.0f : __frcp_rn(vs), 0.0f);
     }
     if (kSparse && page >= 0) f.w = __int_as_float(sel[page0 + i] << p.c.page_shift);   // first position
     s_meta[i] = f;

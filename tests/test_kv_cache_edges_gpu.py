@@ -26,3 +26,73 @@ def test_tiles_into_an_unaligned_output(cuda_lib, dim, page, t, group, dtype):
     room = torch.full((2, 2 * group, t, dim + 5), 7.0, dtype=q.dtype, device="cuda")
     got = K.attention_kv_i8(q, cache, table, _i32(lens), dim ** -0.5, out=room[..., 3: dim + 3])
     assert torch.equal(got, want) and (room[..., :3] == 7).all() and (room[..., dim + 3:] == 7).all()
+
+
+# ---------------------------------------------------------------------------
+# A page with a NaN scale
+# ---------------------------------------------------------------------------
+def _sees(pos, page, size, causal, window):
+    """Whether a row at `pos` (-1: none) sees a key of page ordinal `page`."""
+    first = max(0, pos + 1 - window) if window else 0
+    return pos >= 0 and page * size + size > first and (not causal or page * size <= pos)
+
+
+@pytest.mark.parametrize("t,causal,window", [(1, True, 0), (1, True, 4), (5, True, 4), (9, True, 0), (30, True, 0), (30, True, 7),
+                                             (20, False, 0), (140, True, 0), (140, True, 30)])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_nan_scales_reach_the_rows_that_see_them_alone(cuda_lib, t, causal, window, wide, which):
+    """One page of a sequence takes a NaN scale, for keys or for values: the rows that see a key of it are NaN, the
+    others and the other sequence are what they were."""
+    from h3vae_b200 import kernels as K
+    rng = np.random.default_rng(30 + t)
+    lens, size = [150, 200], 16
+    ref, rows, table = _filled(rng, lens, 2, 64, size)
+    q = torch.from_numpy(rng.standard_normal((2, 4, t, 64))).half().cuda()
+    args = dict(causal=causal, window=window)
+    out, _, bound = _attend_all(ref, rows, q, lens, [t, t], 0.125, size, **args)
+    for page in (9, 8, 3):
+        cache = _cache(ref)
+        getattr(cache, which + "_scale")[rows[0][page]] = float("nan")
+        got = K.attention_kv_i8(q, cache, _wide(table) if wide else table, _i32(lens), 0.125, **args)
+        hit = np.array([_sees(150 - t + i if 150 - t + i >= 0 else -1, page, size, causal, window) for i in range(t)])
+        assert torch.isnan(got[0][:, torch.from_numpy(hit).cuda()]).all()
+        if not hit.all():
+            R.check(got[0][:, torch.from_numpy(~hit).cuda()], out[0][:, ~hit], bound[0][:, ~hit], torch.float16)
+        R.check(got[1], out[1], bound[1], torch.float16)
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_nan_scales_and_rows_without_keys(cuda_lib, which):
+    """Padding rows and rows before the first key are zero, whatever the pages hold."""
+    from h3vae_b200 import kernels as K
+    rng = np.random.default_rng(31)
+    lens, counts, t = [70, 5], [3, 9], 12
+    ref, rows, table = _filled(rng, lens, 1, 64, 16)
+    q = torch.from_numpy(rng.standard_normal((2, 2, t, 64))).half().cuda()
+    cache = _cache(ref)
+    for row in rows:
+        for page in row:
+            getattr(cache, which + "_scale")[page] = float("nan")
+    for tab in (table, _wide(table)):
+        got, lse = K.attention_kv_i8(q, cache, tab, _i32(lens), 0.125, counts=_i32(counts), return_lse=True)
+        assert torch.isnan(got[0, :, :3]).all() and (got[0, :, 3:] == 0).all() and (lse[0, :, 3:] == -np.inf).all()
+        assert (got[1, :, :4] == 0).all() and torch.isnan(got[1, :, 4:9]).all() and (got[1, :, 9:] == 0).all()
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_nan_scales_of_selected_pages_past_a_row(cuda_lib, which):
+    """A selected page that lies behind a row's position adds nothing to it."""
+    from h3vae_b200 import kernels as K
+    rng = np.random.default_rng(32)
+    lens, t, size = [150], 20, 16
+    ref, rows, table = _filled(rng, lens, 2, 64, size)
+    q = torch.from_numpy(rng.standard_normal((1, 4, t, 64))).half().cuda()
+    sel = torch.arange(10, dtype=torch.int32, device="cuda").expand(1, 2, t, 10).contiguous()
+    out, _, bound = _attend_all(ref, rows, q, lens, [t], 0.125, size, selected=sel.cpu().numpy())
+    cache = _cache(ref)
+    getattr(cache, which + "_scale")[rows[0][9]] = float("nan")
+    got = K.attention_kv_i8(q, cache, table, _i32(lens), 0.125, selected=sel)
+    hit = torch.arange(130, 150) >= 144
+    assert torch.isnan(got[:, :, hit.cuda()]).all()
+    R.check(got[:, :, ~hit.cuda()], out[:, :, ~hit.numpy()], bound[:, :, ~hit.numpy()], torch.float16)
