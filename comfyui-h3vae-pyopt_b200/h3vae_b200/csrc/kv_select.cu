@@ -56,21 +56,25 @@ __device__ __forceinline__ void load_sums(const KvSelectParams& p, int page, int
   }
 }
 
-// One query row to codes and their scale, by a warp.
+// One query row to codes and their scale, by a warp.  A row with a NaN or an infinity
+// has no codes: its scale becomes NaN and with it all its scores, which fmaxf over
+// the group then leaves out.
 template <typename T, int D>
 __device__ __forceinline__ void quantise_row(const T* q, uint32_t* codes, float* scale) {
   const int lane = threadIdx.x & 31;
-  float x[D / 32], top = 0.0f;
+  float x[D / 32];
+  uint32_t top = 0;      // magnitudes as bits: their order is the floats', infinities and NaN above all
 #pragma unroll
   for (int e = 0; e < D / 32; ++e) {
     x[e] = to_f32(q[lane * (D / 32) + e]);
-    top = fmaxf(top, fabsf(x[e]));
+    top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
   }
-  const float s = fmaxf(__fmul_rn(warp_max(top), kKvInv127), kKvMinScale), inv = __frcp_rn(s);
+  top = __reduce_max_sync(0xffffffffu, top);
+  const float s = fmaxf(__fmul_rn(__uint_as_float(top), kKvInv127), kKvMinScale), inv = __frcp_rn(s);
 #pragma unroll
   for (int e = 0; e < D / 32; ++e)
     reinterpret_cast<uint8_t*>(codes)[lane * (D / 32) + e] = static_cast<uint8_t>(rint_bits(__fmul_rn(x[e], inv)));
-  if (lane == 0) *scale = s;
+  if (lane == 0) *scale = top > 0x7f7fffffu ? __int_as_float(0x7fffffff) : s;
 }
 
 // A row's product with a page's sums.

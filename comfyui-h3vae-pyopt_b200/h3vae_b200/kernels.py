@@ -901,7 +901,8 @@ def attention_kv_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: t
 def kv_select_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torch.Tensor, pages: int, *,
                  counts: torch.Tensor | None = None) -> torch.Tensor:
     """The `pages` pages each query attends to: its own, and the earlier ones whose summed keys have the largest
-    product with the row-quantised query (the maximum over the group's heads; ties: the lower page).
+    product with the row-quantised query (the maximum over the group's heads, those with a NaN or an infinity left
+    out; ties: the lower page).
     q, lengths, counts as in attention_kv_i8; returns int32 [B, H, T, pages], ascending, -1 where none is left."""
     table, batch, width = _kv_table(cache, page_table)
     heads, tokens, q_strides = _kv_query(q, cache, batch)

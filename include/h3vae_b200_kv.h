@@ -96,7 +96,8 @@ int h3b_attention_kv_i8(const void* q, const int64_t* q_strides, const h3b_kv_ca
  * the earlier (complete) pages those with the highest scores; ties go to the lower page.
  *   row quantisation of every query row: s = max(max|q| * fp32(1/127), 1e-30), q8 = rint(q * (1 / s))
  *   score(page) = max over the group's heads of float(q8 . k_sum[page]) * s, times k_scale[page]
- *   (whole-number products; a NaN score ranks first)
+ *   (whole-number products; the scores of a page whose scale is NaN rank first).  A head whose query row holds a
+ *   NaN or an infinity is left out of the maximum; where no head is left, all pages count alike
  * selected: int32 [batch, kv_heads, tokens, n_selected], ascending ordinals, -1 where no page is left and for
  * rows without a position.  q, lengths and counts as in h3b_attention_kv_i8.
  * Workspace: h3b_kv_select_i8_workspace_size(...) bytes, 16-byte aligned. */

@@ -96,3 +96,33 @@ def test_nan_scales_of_selected_pages_past_a_row(cuda_lib, which):
     hit = torch.arange(130, 150) >= 144
     assert torch.isnan(got[:, :, hit.cuda()]).all()
     R.check(got[:, :, ~hit.cuda()], out[:, :, ~hit.numpy()], bound[:, :, ~hit.numpy()], torch.float16)
+
+
+# ---------------------------------------------------------------------------
+# Selection with NaN and infinities in the queries
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("t,wide", [(1, False), (1, True), (6, False), (12, False)])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_select_leaves_out_heads_that_are_not_finite(cuda_lib, t, wide, dtype):
+    """A head whose query holds a NaN or an infinity has no say in its group's choice; where no head is left, all
+    pages count alike and the lowest are taken."""
+    from h3vae_b200 import kernels as K
+    rng = np.random.default_rng(50 + t)
+    lens, size, n, group = [700, 333], 16, 6, 3
+    ref, rows, table = _filled(rng, lens, 2, 64, size)
+    cache = _cache(ref)
+    table = _wide(table, 5000) if wide else table
+    q = torch.from_numpy(rng.standard_normal((2, 2 * group, t, 64))).to(TYPES[dtype])
+    fine = q.float().numpy().copy()
+    q[0, 0, :, 5] = float("nan")
+    q[0, 2, :, 63] = float("inf")
+    q[0, 4, :, 0] = -float("inf")
+    q[1, 3:, t - 1, 17] = float("nan")
+    got = K.kv_select_i8(q.cuda(), cache, table, _i32(lens), n).cpu().numpy()
+    left = {(0, 0): [1], (0, 1): [3, 5], (1, 0): [0, 1, 2], (1, 1): [3, 4, 5]}
+    for (b, h), heads in left.items():
+        pos = [lens[b] - t + i for i in range(t)]
+        want = R.select(fine[b, heads], ref.scale["k"][rows[b], h], ref.k_sum[rows[b], h], pos, n, size, len(heads))
+        if (b, h) == (1, 1):
+            want[t - 1] = [*range(n - 1), pos[-1] // size]
+        assert np.array_equal(got[b, h], want), (b, h)
