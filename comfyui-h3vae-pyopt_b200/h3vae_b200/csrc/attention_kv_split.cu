@@ -51,10 +51,12 @@ struct KvSplit {
   static constexpr int kSmem = kRing + kMeta + kSplitWarps * kSplitStages * 8 + 128;
 };
 
-// Tiles a sequence's rows need, in tiles of `keys`.
+// Tiles a sequence's rows need, in tiles of `keys`: none without queries.
 __device__ __forceinline__ int split_tiles(const KvAttnParams& p, int b, int keys, int& tile0) {
   const int len = kv_length(p.c, p.lengths, b), n = kv_count(p.counts, p.tokens, b);
   int first, last, unused;
+  tile0 = 0;
+  if (n == 0) return 0;
   const int t0 = max(0, n - len);             // the first row that has a position
   kv_range(p, len, n, t0, first, unused);
   kv_range(p, len, n, n - 1, unused, last);
@@ -189,6 +191,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_s
     if (split == 0 && tid == 0 && hk == 0 && rt == 0 && p.plan) p.plan[b] = make_int2(first_slot, splits);
   }
   const int len = kv_length(p.c, p.lengths, b), n_tok = kv_count(p.counts, p.tokens, b);
+  if ((kSparse ? t_sparse : rt * kSplitRows / p.group) >= n_tok) tile1 = tile0;      // padding rows see nothing
 
   // ---- the pages of the run: numbers, then the first copies, then scales ----
   const int page0 = (tile0 * KT) >> p.c.page_shift;

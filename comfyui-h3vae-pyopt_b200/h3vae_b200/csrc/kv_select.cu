@@ -29,16 +29,21 @@ struct KvSelectParams {
   int group, tokens, n, row_keys;
 };
 
-// Last page ordinal row t of sequence b sees, -1 if none.
+// Query tokens of sequence b.
+__device__ __forceinline__ int kv_queries(const KvSelectParams& p, int b) {
+  return p.counts ? max(0, min(p.counts[b], p.tokens)) : p.tokens;
+}
+
+// Last page ordinal row t of sequence b sees, -1 if none (t = -1, a sequence without queries, among them).
 __device__ __forceinline__ int kv_last_page(const KvSelectParams& p, int b, int t) {
   int len = max(p.lengths[b], 0);
   if (len > p.c.width * p.c.page) {
     record_error(kErrKvPage);
     len = p.c.width * p.c.page;
   }
-  const int n = p.counts ? min(p.counts[b], p.tokens) : p.tokens;
+  const int n = kv_queries(p, b);
   const int pos = len - n + t;
-  return t >= n || pos < 0 ? -1 : pos >> p.c.page_shift;
+  return t < 0 || t >= n || pos < 0 ? -1 : pos >> p.c.page_shift;
 }
 
 constexpr int kSelThreads = 128;
@@ -106,7 +111,8 @@ __global__ void __launch_bounds__(kSelThreads) kv_score_kernel(const KvSelectPar
   __shared__ float s_s[kSelRows];
   const int head = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5;
   const int slot = blockIdx.x * kSelThreads + threadIdx.x;
-  const int last = kv_last_page(p, b, (p.counts ? min(p.counts[b], p.tokens) : p.tokens) - 1);
+  const int tokens = kv_queries(p, b);
+  const int last = kv_last_page(p, b, tokens - 1);
   if (static_cast<int>(blockIdx.x) * kSelThreads >= last) return;   // no complete page here (uniform)
   uint32_t k[D / 2];
   float k_scale = 0.0f;
@@ -115,8 +121,8 @@ __global__ void __launch_bounds__(kSelThreads) kv_score_kernel(const KvSelectPar
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int per = max(1, kSelRows / p.group);      // query tokens per round
   float best = 0.0f;
-  for (int t0 = 0; t0 < p.tokens; t0 += per) {
-    const int t1 = min(t0 + per, p.tokens);
+  for (int t0 = 0; t0 < tokens; t0 += per) {      // padding rows have no keys, and none are looked for
+    const int t1 = min(t0 + per, tokens);
     for (int g0 = 0; g0 < p.group; g0 += kSelRows) {   // groups wider than the buffer take several rounds
       const int g1 = min(g0 + kSelRows, p.group), gn = g1 - g0, rows = (t1 - t0) * gn;
       __syncthreads();
@@ -298,12 +304,13 @@ __global__ void __launch_bounds__(kThreads) kv_select_kernel(const KvSelectParam
   const int rank = blockIdx.x, blocks = gridDim.x, head = blockIdx.y, b = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5;
   cluster_arrive();   // waited for below: all blocks run
-  const int end = kv_last_page(p, b, (p.counts ? min(p.counts[b], p.tokens) : p.tokens) - 1);   // complete pages
+  const int tokens = kv_queries(p, b);
+  const int end = kv_last_page(p, b, tokens - 1);   // complete pages
   int slot = rank * kThreads + tid, page = slot < end ? kv_page(p.c, b, slot) : -1;
   uint32_t k[D / 2];
   float k_scale = 0.0f;
   if (page >= 0) load_sums<D>(p, page, head, k, k_scale);
-  const int rows = p.tokens * p.group;
+  const int rows = tokens * p.group;
   for (int r = warp; r < rows; r += kThreads / 32) {
     const int t = r / p.group, h = head * p.group + r % p.group;
     quantise_row<T, D>(static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1] + t * p.qs[2], s_q[r], &s_s[r]);
@@ -312,7 +319,7 @@ __global__ void __launch_bounds__(kThreads) kv_select_kernel(const KvSelectParam
   cluster_wait();
   const uint32_t base = smem_u32(s_keys);
   while (slot < end) {
-    for (int t = 0; t < p.tokens; ++t) {
+    for (int t = 0; t < tokens; ++t) {
       uint32_t key = 0;                                  // a bad page number: never worth choosing
       if (page >= 0) {
         float best = row_score<D>(k, s_q[t * p.group], s_s[t * p.group]);

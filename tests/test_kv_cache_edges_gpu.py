@@ -126,3 +126,35 @@ def test_select_leaves_out_heads_that_are_not_finite(cuda_lib, t, wide, dtype):
         if (b, h) == (1, 1):
             want[t - 1] = [*range(n - 1), pos[-1] // size]
         assert np.array_equal(got[b, h], want), (b, h)
+
+
+# ---------------------------------------------------------------------------
+# Sequences without queries
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("t,group,wide", [(1, 1, False), (1, 4, True), (7, 2, False), (40, 1, True), (140, 1, True)])
+def test_sequences_without_queries_are_not_looked_at(cuda_lib, t, group, wide):
+    """A count of zero: zero rows, and no page of the sequence is looked up (its table holds no page numbers, which a
+    lookup would report)."""
+    from h3vae_b200 import _lib, kernels as K
+    rng = np.random.default_rng(40 + t)
+    lens, counts = [500, 700, 333], [t, 0, max(0, t - 1)]
+    ref, rows, table = _filled(rng, lens, 2, 64, 16)
+    cache = _cache(ref)
+    table = _wide(table) if wide else table
+    q = torch.from_numpy(rng.standard_normal((3, 2 * group, t, 64))).half().cuda()
+    args = dict(counts=_i32(counts))
+    want = K.attention_kv_i8(q, cache, table, _i32(lens), 0.125, **args)
+    pages = K.kv_select_i8(q, cache, table, _i32(lens), 4, **args)
+    kept = K.attention_kv_i8(q, cache, table, _i32(lens), 0.125, selected=pages, **args)
+    assert _lib.device_error() == 0
+    gone = table.clone()
+    gone[1] = -1
+    got, lse = K.attention_kv_i8(q, cache, gone, _i32(lens), 0.125, return_lse=True, **args)
+    assert _lib.device_error() == 0
+    assert torch.equal(got, want) and (got[1] == 0).all() and (lse[1] == -np.inf).all()
+    assert torch.equal(K.kv_select_i8(q, cache, gone, _i32(lens), 4, **args), pages) and (pages[1] == -1).all()
+    assert _lib.device_error() == 0
+    every = torch.arange(4, dtype=torch.int32, device="cuda").expand(1, 2, t, 4)     # pages named for rows that are none
+    sel = torch.cat([pages[:1], every, pages[2:]]).contiguous()
+    assert torch.equal(K.attention_kv_i8(q, cache, gone, _i32(lens), 0.125, selected=sel, **args), kept)
+    assert _lib.device_error() == 0
