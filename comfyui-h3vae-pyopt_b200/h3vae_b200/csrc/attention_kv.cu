@@ -31,6 +31,7 @@ struct KvPlan {
 KvPlan kv_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens, int64_t dim, int64_t width,
                int64_t page, int64_t n_selected) {
   using namespace h3b;
+  using h3b_host::kv_bytes;
   KvPlan k{};
   k.join_warps = 1;
   const int64_t group = q_heads / kv_heads;
@@ -44,7 +45,7 @@ KvPlan kv_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens,
     k.row_tiles = (rows + 2 * kKtRows - 1) / (2 * kKtRows);
     const int64_t blocks = batch * kv_heads * k.row_tiles, most_blocks = (width * page + kKtKeys - 1) / kKtKeys;
     k.slots = std::max<int64_t>(1, std::min(h3b_host::num_sms() / blocks, most_blocks / 4));
-    k.part_bytes = k.slots > 1 ? (size_t)(k.slots * batch * kv_heads * rows) * (dim + 4) * 4 : 0;
+    k.part_bytes = k.slots > 1 ? kv_bytes({k.slots, batch, kv_heads, rows, dim + 4, 4}) : 0;
     k.join_warps = k.slots >= 4 ? 4 : 1;
     return k;
   }
@@ -70,7 +71,7 @@ KvPlan kv_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens,
     k.chunk = std::min(most, (tiles + want - 1) / want);
     k.slots = (tiles + k.chunk - 1) / k.chunk;
     k.join_warps = k.slots >= 4 ? 4 : 1;
-    k.part_bytes = k.slots > 1 ? (size_t)(batch * tokens * k.slots) * kv_heads * k.row_tiles * kSplitRows * (dim + 4) * 4 : 0;
+    k.part_bytes = k.slots > 1 ? kv_bytes({batch, tokens, k.slots, kv_heads, k.row_tiles, kSplitRows, dim + 4, 4}) : 0;
   } else {
     k.chunk = most;
     const int64_t per = kv_heads * k.row_tiles;
@@ -88,7 +89,7 @@ KvPlan kv_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens,
     k.slots = std::max(k.fit, batch + batch * (tiles / most));
     k.plan_bytes = k.slots > batch ? ((size_t)batch * 8 + 15) & ~size_t(15) : 0;
     k.join_warps = k.slots >= 4 * batch ? 4 : 1;   // 56 parts of a row: the call takes 60 us with four, 75 with one
-    k.part_bytes = k.slots > batch ? (size_t)k.slots * kv_heads * k.row_tiles * kSplitRows * (dim + 4) * 4 : 0;
+    k.part_bytes = k.slots > batch ? kv_bytes({k.slots, kv_heads, k.row_tiles, kSplitRows, dim + 4, 4}) : 0;
   }
   return k;
 }
@@ -183,11 +184,13 @@ int launch_kv_attention(const char* name, const h3b::KvAttnParams& p, bool tile,
 extern "C" size_t h3b_attention_kv_i8_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens,
                                                      int64_t head_dim, int64_t table_width, int64_t page_size,
                                                      int64_t n_selected) {
-  if (batch <= 0 || kv_heads <= 0 || q_heads < kv_heads || tokens <= 0 || table_width <= 0 || page_size < 16 ||
-      (head_dim != 64 && head_dim != 128))
-    return 16;
+  using namespace h3b_host;
+  if (batch <= 0 || batch > kKvMostBatch || kv_heads <= 0 || q_heads < kv_heads || q_heads > kKvMostHeads || tokens <= 0 ||
+      tokens > kKvMostKeys / q_heads || page_size < 16 || page_size > 128 || table_width <= 0 ||
+      table_width > kKvMostKeys / page_size || n_selected > kKvMostSelected || (head_dim != 64 && head_dim != 128))
+    return 16;   // the call refuses these
   const KvPlan k = kv_plan(batch, q_heads, kv_heads, tokens, head_dim, table_width, page_size, n_selected);
-  return 16 + k.plan_bytes + k.part_bytes;
+  return k.part_bytes > SIZE_MAX - 16 - k.plan_bytes ? SIZE_MAX : 16 + k.plan_bytes + k.part_bytes;
 }
 
 extern "C" int h3b_attention_kv_i8(const void* q, const int64_t* q_strides, const h3b_kv_cache* cache,
@@ -203,16 +206,17 @@ extern "C" int h3b_attention_kv_i8(const void* q, const int64_t* q_strides, cons
   if (!q || !out || !q_strides || !out_strides || !lengths) return h3b_host::set_error(H3B_EINVAL, "%s: NULL argument", name);
   if (dtype != H3B_TYPE_F16 && dtype != H3B_TYPE_BF16)
     return h3b_host::set_error(H3B_EINVAL, "%s: q must be fp16 or bf16", name);
-  if (q_heads <= 0 || q_heads % cache->kv_heads || q_heads > 65535)
+  if (q_heads <= 0 || q_heads % cache->kv_heads || q_heads > h3b_host::kKvMostHeads)
     return h3b_host::set_error(H3B_EINVAL, "%s: q_heads must be a positive multiple of kv_heads", name);
-  if (tokens < 0 || tokens * q_heads > (int64_t(1) << 30))
+  if (tokens < 0 || tokens > h3b_host::kKvMostKeys / q_heads)
     return h3b_host::set_error(H3B_EINVAL, "%s: bad token count", name);
   if (window < 0 || (window > 0 && !causal)) return h3b_host::set_error(H3B_EINVAL, "%s: a window needs causal", name);
-  if (selected && (n_selected <= 0 || n_selected > (int64_t(1) << 20) || !causal || window > 0))
+  if (selected && (n_selected <= 0 || n_selected > h3b_host::kKvMostSelected || !causal || window > 0))
     return h3b_host::set_error(H3B_EINVAL, "%s: selected pages need causal, no window and 1 to 2^20 pages", name);
   if (tokens == 0) return H3B_OK;
   const KvPlan k = kv_plan(batch, q_heads, cache->kv_heads, tokens, cache->head_dim, table_width, cache->page_size,
                            selected ? n_selected : 0);
+  if (k.part_bytes > SIZE_MAX / 2 || k.slots > INT32_MAX) return h3b_host::set_error(H3B_EUNSUPPORTED, "%s: problem too large", name);
   const size_t need = k.plan_bytes + k.part_bytes;
   if (need && (!workspace || !h3b_host::aligned16(workspace) || workspace_bytes < 16 + need))
     return h3b_host::set_error(H3B_EINVAL, "%s: workspace missing, misaligned or too small", name);

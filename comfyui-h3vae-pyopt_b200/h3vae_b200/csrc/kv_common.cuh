@@ -123,6 +123,18 @@ __device__ __forceinline__ uint2 quantise8(float (&x)[8], float f) {
 
 namespace h3b_host {
 
+// Largest sizes of a call: grid dimensions, and positions that fit 32 bits.
+constexpr int64_t kKvMostBatch = 65535, kKvMostHeads = 65535, kKvMostKeys = int64_t(1) << 30;
+constexpr int64_t kKvMostSelected = int64_t(1) << 20;
+
+// The product of sizes, or SIZE_MAX where that does not fit.
+inline size_t kv_bytes(std::initializer_list<int64_t> sizes) {
+  size_t n = 1;
+  for (const int64_t s : sizes)
+    if (__builtin_mul_overflow(n, static_cast<size_t>(s), &n)) return SIZE_MAX;
+  return n;
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Checks the cache and table arguments every entry point shares and fills the device view.
@@ -139,8 +151,8 @@ inline int kv_view(const char* name, const h3b_kv_cache* c, const int32_t* table
                      (long long)c->page_size);
   if (batch <= 0 || width <= 0 || c->num_pages <= 0 || c->kv_heads <= 0)
     return set_error(H3B_EINVAL, "%s: batch, table width, pages and heads must be positive", name);
-  if (batch > 65535 || c->kv_heads > 65535 || c->num_pages > (int64_t(1) << 30) ||
-      width * c->page_size > (int64_t(1) << 30))
+  if (batch > kKvMostBatch || c->kv_heads > kKvMostHeads || c->num_pages > (int64_t(1) << 30) ||
+      width > kKvMostKeys / c->page_size)
     return set_error(H3B_EUNSUPPORTED, "%s: problem too large", name);
   view->code[0] = c->k;
   view->code[1] = c->v;

@@ -373,7 +373,8 @@ int launch_kv_select(const char* name, const h3b::KvSelectParams& p, int blocks,
 extern "C" size_t h3b_kv_select_i8_workspace_size(int64_t batch, int64_t kv_heads, int64_t tokens,
                                                   int64_t table_width) {
   if (batch <= 0 || kv_heads <= 0 || tokens <= 0 || table_width <= 0) return 16;
-  return (size_t)batch * kv_heads * tokens * ((table_width + 3) & ~int64_t(3)) * 4;
+  if (table_width > h3b_host::kKvMostKeys) return SIZE_MAX;
+  return h3b_host::kv_bytes({batch, kv_heads, tokens, (table_width + 3) & ~int64_t(3), 4});
 }
 
 extern "C" int h3b_kv_select_i8(const void* q, const int64_t* q_strides, const h3b_kv_cache* cache,
@@ -387,9 +388,9 @@ extern "C" int h3b_kv_select_i8(const void* q, const int64_t* q_strides, const h
   if (!q || !q_strides || !lengths || !selected) return h3b_host::set_error(H3B_EINVAL, "%s: NULL argument", name);
   if (dtype != H3B_TYPE_F16 && dtype != H3B_TYPE_BF16)
     return h3b_host::set_error(H3B_EINVAL, "%s: q must be fp16 or bf16", name);
-  if (q_heads <= 0 || q_heads % cache->kv_heads || q_heads > 65535)
+  if (q_heads <= 0 || q_heads % cache->kv_heads || q_heads > h3b_host::kKvMostHeads)
     return h3b_host::set_error(H3B_EINVAL, "%s: q_heads must be a positive multiple of kv_heads", name);
-  if (tokens < 0 || tokens > (int64_t(1) << 20) || n_selected <= 0 || n_selected > (int64_t(1) << 20))
+  if (tokens < 0 || tokens > (int64_t(1) << 20) || n_selected <= 0 || n_selected > h3b_host::kKvMostSelected)
     return h3b_host::set_error(H3B_EINVAL, "%s: bad token count or page count", name);
   if (tokens == 0) return H3B_OK;
   if (!workspace || !h3b_host::aligned16(workspace) ||
