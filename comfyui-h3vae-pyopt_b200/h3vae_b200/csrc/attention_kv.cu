@@ -1,8 +1,6 @@
 // Host side of attention over the paged INT8 cache: the choice between the
 // kernels of attention_kv_split.cu and attention_kv_tile.cu, workspaces, checks.
-#include <mutex>
-#include <set>
-#include <utility>
+#include <atomic>
 
 #include "attention_kv.cuh"
 
@@ -94,17 +92,16 @@ KvPlan kv_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens,
   return k;
 }
 
-// Lets `kernel` use `bytes` of shared memory; asked of the driver once per kernel and device.
-int allow_smem(const char* name, const void* kernel, int bytes) {
-  static std::mutex lock;
-  static std::set<std::pair<const void*, int>> done;
+// Lets `kernel` use `bytes` of shared memory; asked of the driver once per kernel and device (`done`: a bit for each
+// of the first 64 devices; a kernel's own word).  Nothing here throws: the C entries have no caller that could catch it.
+int allow_smem(const char* name, const void* kernel, int bytes, std::atomic<uint64_t>& done) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  std::lock_guard<std::mutex> guard(lock);
-  if (e == cudaSuccess && done.count({kernel, dev})) return H3B_OK;
+  const uint64_t bit = dev >= 0 && dev < 64 ? uint64_t(1) << dev : 0;
+  if (e == cudaSuccess && (done.load(std::memory_order_relaxed) & bit)) return H3B_OK;
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return h3b_host::set_error(H3B_ECUDA, "%s: smem attribute: %s", name, cudaGetErrorString(e));
-  done.insert({kernel, dev});
+  done.fetch_or(bit, std::memory_order_relaxed);
   return H3B_OK;
 }
 
@@ -132,7 +129,8 @@ int launch_kv_split(const char* name, const h3b::KvAttnParams& p, int64_t batch,
   const int rows = kSparse ? p.group : p.group * p.tokens;
   auto kernel = rows <= 8 ? attention_kv_split_kernel<T, D, kSparse, true> : attention_kv_split_kernel<T, D, kSparse, false>;
   constexpr int smem = KvSplit<D>::kSmem;
-  int rc = allow_smem(name, reinterpret_cast<const void*>(kernel), smem);
+  static std::atomic<uint64_t> allowed[2];
+  int rc = allow_smem(name, reinterpret_cast<const void*>(kernel), smem, allowed[rows <= 8]);
   if (rc) return rc;
   const int64_t x = (int64_t)p.slots * p.row_tiles * (kSparse ? p.tokens : 1);
   if (x > 0x7fffffff) return h3b_host::set_error(H3B_EUNSUPPORTED, "%s: problem too large", name);
@@ -165,7 +163,8 @@ int launch_kv_tile(const char* name, const h3b::KvAttnParams& p, int64_t batch, 
   auto kernel = attention_kv_tile_kernel<T, D>;
   constexpr int smem = KvTile<D>::kSmem;
   static_assert(smem <= 232448, "shared memory budget");
-  int rc = allow_smem(name, reinterpret_cast<const void*>(kernel), smem);
+  static std::atomic<uint64_t> allowed;
+  int rc = allow_smem(name, reinterpret_cast<const void*>(kernel), smem, allowed);
   if (rc) return rc;
   kernel<<<dim3((unsigned)(p.row_tiles * p.slots), (unsigned)p.c.heads, (unsigned)batch), kKtThreads, smem, st>>>(p);
   rc = h3b_host::check_launch(name);

@@ -43,3 +43,11 @@ def test_warps_stay_whole_around_loads_from_tensor_memory():
         body = code[call.end():]
         body = body[: min((body.find(x) for x in ("\n}", "#pragma unroll 1") if x in body), default=len(body))]
         assert "continue;" not in body, body[:200]
+
+
+def test_nothing_throws_at_the_c_entries():
+    """A C++ exception that leaves an extern "C" function ends the process: nothing that allocates or locks by throwing."""
+    for path in SOURCES:
+        code = _code(path)
+        assert not re.search(r"std::(set|map|vector|string|function|mutex|lock_guard|unordered_\w+|call_once)\b", code), path.name
+        assert not re.search(r"\b(throw|new)\b", code), path.name
