@@ -56,8 +56,9 @@ def _kv_stream(device: torch.device) -> int:
 
 
 @functools.lru_cache(maxsize=256)
-def _kv_workspace_bytes(name: str, *sizes: int) -> int:
-    """Bytes that the library's `name`_workspace_size asks for (a function of sizes alone)."""
+def _kv_workspace_bytes(name: str, device_index: int | None, *sizes: int) -> int:
+    """Bytes that the library's `name`_workspace_size asks for: a function of the sizes and of the current device
+    (the plan goes by its SMs), whose index makes answers for different devices different entries."""
     return int(getattr(_lib.load(), name + "_workspace_size")(*sizes))
 
 
@@ -886,7 +887,7 @@ def attention_kv_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: t
     lse = torch.empty((batch, heads, tokens), device=dev, dtype=F32) if return_lse else None
     if tokens:
         lib = _lib.load()
-        ws_bytes = _kv_workspace_bytes("h3b_attention_kv_i8", batch, heads, cache.kv_heads, tokens, dim, width,
+        ws_bytes = _kv_workspace_bytes("h3b_attention_kv_i8", dev.index, batch, heads, cache.kv_heads, tokens, dim, width,
                                        cache.page_size, n_sel)
         ws = cache.k.new_empty(ws_bytes) if ws_bytes > 16 else None      # 16: the call needs none
         _lib.check(lib.h3b_attention_kv_i8(
@@ -912,7 +913,7 @@ def kv_select_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torc
     selected = page_table.new_empty((batch, cache.kv_heads, tokens, pages))
     if tokens:
         lib = _lib.load()
-        ws_bytes = _kv_workspace_bytes("h3b_kv_select_i8", batch, cache.kv_heads, tokens, width)
+        ws_bytes = _kv_workspace_bytes("h3b_kv_select_i8", dev.index, batch, cache.kv_heads, tokens, width)
         ws = cache.k.new_empty(ws_bytes)
         _lib.check(lib.h3b_kv_select_i8(
             q.data_ptr(), q_strides, cache.struct, table, batch, width, _kv_index(lengths, "lengths", (batch,), dev),

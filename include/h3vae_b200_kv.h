@@ -80,8 +80,9 @@ int h3b_kv_read_i8(const h3b_kv_cache* cache, const int32_t* page_table, int64_t
  *   lse        NULL, or fp32 [batch, q_heads, tokens]: the natural logarithm of each row's sum of exp
  * Rows that see no key (padding, an empty sequence, a position before the first key) are zero with lse
  * -infinity.  Keys a row does not see have no effect on it, whatever their page holds.
- * Workspace: h3b_attention_kv_i8_workspace_size(...) bytes of the same sizes, 16-byte aligned; contents are not
- * kept between calls.  Where that is 16 the call needs none and takes NULL. */
+ * Workspace: h3b_attention_kv_i8_workspace_size(...) bytes of the same sizes, asked for with the same current
+ * device (the plan goes by its number of SMs), 16-byte aligned; contents are not kept between calls.  Where that is
+ * 16 the call needs none and takes NULL. */
 size_t h3b_attention_kv_i8_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens,
                                           int64_t head_dim, int64_t table_width, int64_t page_size,
                                           int64_t n_selected);
