@@ -7,6 +7,7 @@ These are the only functions in the package that touch the native library.
 """
 from __future__ import annotations
 
+import contextlib
 import functools
 import struct
 
@@ -53,6 +54,17 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 def _kv_stream(device: torch.device) -> int:
     return _stream(device) if _raw_stream is None or device.index is None else _raw_stream(device.index)
+
+
+# The current device's index without a check that CUDA is up, where torch has the call.
+_device_index = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_STAY = contextlib.nullcontext()
+
+
+def _kv_device(device: torch.device):
+    """The cache's device as the current one: the library launches on the current device and plans for its SMs, and a
+    default stream has the same handle on every device."""
+    return _STAY if device.index is None or device.index == _device_index() else torch.cuda.device(device)
 
 
 @functools.lru_cache(maxsize=256)
@@ -816,10 +828,11 @@ def kv_write_i8(cache, page_table: torch.Tensor, start: torch.Tensor, k: torch.T
     dev = cache.device
     if not k.shape[2]:
         return
-    _lib.check(_lib.load().h3b_kv_write_i8(
-        cache.struct, table, batch, width, _kv_index(start, "start", (batch,), dev),
-        _kv_index(counts, "counts", (batch,), dev), k.data_ptr(), k_strides, v.data_ptr(), v_strides, k.shape[2],
-        _KV_TYPES[k.dtype], _kv_stream(dev)))
+    with _kv_device(dev):
+        _lib.check(_lib.load().h3b_kv_write_i8(
+            cache.struct, table, batch, width, _kv_index(start, "start", (batch,), dev),
+            _kv_index(counts, "counts", (batch,), dev), k.data_ptr(), k_strides, v.data_ptr(), v_strides, k.shape[2],
+            _KV_TYPES[k.dtype], _kv_stream(dev)))
     _count(1)
 
 
@@ -836,10 +849,11 @@ def kv_read_i8(cache, page_table: torch.Tensor, lengths: torch.Tensor, tokens: i
     k = torch.empty((batch, cache.kv_heads, tokens, cache.head_dim), device=dev, dtype=dtype)
     v = torch.empty_like(k)
     if tokens:
-        _lib.check(_lib.load().h3b_kv_read_i8(
-            cache.struct, table, batch, width, _kv_index(start, "start", (batch,), dev),
-            _kv_index(lengths, "lengths", (batch,), dev), k.data_ptr(), v.data_ptr(), tokens, _KV_TYPES[dtype],
-            _kv_stream(dev)))
+        with _kv_device(dev):
+            _lib.check(_lib.load().h3b_kv_read_i8(
+                cache.struct, table, batch, width, _kv_index(start, "start", (batch,), dev),
+                _kv_index(lengths, "lengths", (batch,), dev), k.data_ptr(), v.data_ptr(), tokens, _KV_TYPES[dtype],
+                _kv_stream(dev)))
         _count(1)
     return k, v
 
@@ -887,14 +901,15 @@ def attention_kv_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: t
     lse = torch.empty((batch, heads, tokens), device=dev, dtype=F32) if return_lse else None
     if tokens:
         lib = _lib.load()
-        ws_bytes = _kv_workspace_bytes("h3b_attention_kv_i8", dev.index, batch, heads, cache.kv_heads, tokens, dim, width,
-                                       cache.page_size, n_sel)
-        ws = cache.k.new_empty(ws_bytes) if ws_bytes > 16 else None      # 16: the call needs none
-        _lib.check(lib.h3b_attention_kv_i8(
-            q.data_ptr(), q_strides, cache.struct, table, batch, width, _kv_index(lengths, "lengths", (batch,), dev),
-            _kv_index(counts, "counts", (batch,), dev), heads, tokens, float(scale), 1 if causal else 0, window,
-            _ptr(selected), n_sel, _KV_TYPES[q.dtype], out.data_ptr(), out_strides, _ptr(lse), _ptr(ws),
-            ws_bytes, _kv_stream(dev)))
+        with _kv_device(dev):
+            ws_bytes = _kv_workspace_bytes("h3b_attention_kv_i8", dev.index, batch, heads, cache.kv_heads, tokens, dim, width,
+                                           cache.page_size, n_sel)
+            ws = cache.k.new_empty(ws_bytes) if ws_bytes > 16 else None      # 16: the call needs none
+            _lib.check(lib.h3b_attention_kv_i8(
+                q.data_ptr(), q_strides, cache.struct, table, batch, width, _kv_index(lengths, "lengths", (batch,), dev),
+                _kv_index(counts, "counts", (batch,), dev), heads, tokens, float(scale), 1 if causal else 0, window,
+                _ptr(selected), n_sel, _KV_TYPES[q.dtype], out.data_ptr(), out_strides, _ptr(lse), _ptr(ws),
+                ws_bytes, _kv_stream(dev)))
         _count(1)
     return (out, lse) if return_lse else out
 
@@ -913,11 +928,12 @@ def kv_select_i8(q: torch.Tensor, cache, page_table: torch.Tensor, lengths: torc
     selected = page_table.new_empty((batch, cache.kv_heads, tokens, pages))
     if tokens:
         lib = _lib.load()
-        ws_bytes = _kv_workspace_bytes("h3b_kv_select_i8", dev.index, batch, cache.kv_heads, tokens, width)
-        ws = cache.k.new_empty(ws_bytes)
-        _lib.check(lib.h3b_kv_select_i8(
-            q.data_ptr(), q_strides, cache.struct, table, batch, width, _kv_index(lengths, "lengths", (batch,), dev),
-            _kv_index(counts, "counts", (batch,), dev), heads, tokens, pages, _KV_TYPES[q.dtype], selected.data_ptr(),
-            ws.data_ptr(), ws_bytes, _kv_stream(dev)))
+        with _kv_device(dev):
+            ws_bytes = _kv_workspace_bytes("h3b_kv_select_i8", dev.index, batch, cache.kv_heads, tokens, width)
+            ws = cache.k.new_empty(ws_bytes)
+            _lib.check(lib.h3b_kv_select_i8(
+                q.data_ptr(), q_strides, cache.struct, table, batch, width, _kv_index(lengths, "lengths", (batch,), dev),
+                _kv_index(counts, "counts", (batch,), dev), heads, tokens, pages, _KV_TYPES[q.dtype], selected.data_ptr(),
+                ws.data_ptr(), ws_bytes, _kv_stream(dev)))
         _count(1)
     return selected

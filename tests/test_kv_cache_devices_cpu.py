@@ -89,3 +89,13 @@ def test_workspaces_are_those_of_the_device(two_devices):
         two_devices.current[0] = index
         _calls(index)
     assert two_devices.workspaces == [1000] * 2 + [2000] * 2 + [1000] * 2
+
+
+def test_calls_launch_on_the_device_of_the_cache(two_devices):
+    """With another device current, every call runs on the cache's and leaves the current one as it was."""
+    for current, index in ((0, 1), (1, 0), (1, 1)):
+        two_devices.current[0] = current
+        two_devices.launched.clear()
+        _calls(index)
+        assert [d for _, d in two_devices.launched] == [index] * 4 and two_devices.current[0] == current
+    assert two_devices.workspaces == [2000] * 2 + [1000] * 2 + [2000] * 2
