@@ -9,6 +9,15 @@
 // they are whole numbers, exact in fp16, so the only rounding of the inputs is
 // that of w to fp16, and scales that differ by any factor between pages stay
 // relative to the largest weighted one.
+//
+// The sum of w_j / vs = 2^(q.k - m) has to hold keys whose w_j is below fp32's
+// range, those of a page of zeros (vs = 1e-30) beside one of large values first of
+// all.  So pages with vs < kKvLowScale are summed from the scores, without w_j, where
+// any are met; and where m moves from such pages to others the sum is rescaled in two
+// steps of half the way, since 2^(m - m') alone may be below the range.  Keys from
+// 2^-26 of the largest weight up then count for values up to 2^77; smaller values
+// leave more.  In place of 1 / vs such a page has log2 vs < -30: what the usual sum
+// adds with that, at most 100 w_j, is 1e-7 of the w_j / vs > 2^30 w_j that belongs there.
 #pragma once
 
 #include "kv_common.cuh"
@@ -17,6 +26,7 @@ namespace h3b {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kKvLowScale = 0x1p-30f;   // a page of |v| < 1.2e-7
 
 struct KvAttnParams {
   KvView c;
@@ -68,6 +78,12 @@ __device__ __forceinline__ uint32_t codes_to_h2(uint32_t biased, uint32_t select
   const uint32_t w = __byte_perm(biased, 0x64646464u, selector);
   const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&w), __floats2half2_rn(1152.0f, 1152.0f));
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// l 2^d, for d down to -inf: a sum of weights that is rescaled (the product may be in range where 2^d is not).
+__device__ __forceinline__ float rescale_sum(float l, float d) {
+  const float h = ex2_approx(0.5f * d);
+  return __fmul_rn(__fmul_rn(l, h), h);
 }
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }

@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_s
   using S = KvSplit<D>;
   constexpr int KT = S::kKeys, kTiles = KT / 8, kSteps = D / 16, kThreads = 32 * kSplitWarps;
   extern __shared__ __align__(128) uint8_t smem[];
-  float4* s_meta = reinterpret_cast<float4*>(smem + S::kRing);                 // per page: x scale, log2 vs, 1/vs
+  float4* s_meta = reinterpret_cast<float4*>(smem + S::kRing);                 // per page: x scale, log2 vs, 1/vs or log2 vs
   int* s_page = reinterpret_cast<int*>(s_meta + kSplitPages);                  // pool page, -1: none
   uint64_t* s_bar = reinterpret_cast<uint64_t*>(s_page + kSplitPages);
 
@@ -240,6 +240,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_s
     const int tile = tile0 + warp + s * kSplitWarps;
     if (tile < tile1) issue(tile, s);
   }
+  bool low = false;
   for (int i = tid; i < n_pages; i += kThreads) {
     const int page = s_page[i];
     float4 f = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);   // no page: weight 0
@@ -250,6 +251,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_s
       // a NaN scale of V goes with the scores, which are masked, and not with the factor of the sums, which is not:
       // rows that do not see the page add 0 * (1 / vs)
       f = make_float4(p.c.scale[0][ph] * p.scale_log2, log2f(vs), isnan(vs) ? 0.0f : __frcp_rn(vs), 0.0f);
+      if (vs < kKvLowScale) low = true, f.z = f.y;         // its keys are summed from their scores
     }
     if (kSparse && page >= 0) f.w = __int_as_float(sel[page0 + i] << p.c.page_shift);   // first position
     s_meta[i] = f;
@@ -301,7 +303,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_s
     first_max = max(first_max, __shfl_xor_sync(0xffffffffu, first_max, o));
     last_min = min(last_min, __shfl_xor_sync(0xffffffffu, last_min, o));
   }
-  __syncthreads();   // scales are in shared memory
+  low = __syncthreads_or(low);   // scales are in shared memory
 
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
   float o[D / 8][4];
@@ -362,8 +364,8 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_s
       }
     }
     float ref[2];
-    bool moved = false;
-    float alpha[2];
+    bool moved = low;      // (a run with low pages always goes there)
+    float fall[2], alpha[2];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 1));
@@ -371,18 +373,29 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_s
       const float m_new = fmaxf(m[u], top[u]);
       ref[u] = m_new == -INFINITY ? 0.0f : m_new;
       moved |= m_new > m[u];
-      alpha[u] = ex2_approx(m[u] - ref[u]);
+      fall[u] = m[u] - ref[u];
+      alpha[u] = ex2_approx(fall[u]);
       m[u] = m_new;
     }
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-      for (int u = 0; u < kU; ++u) l[u] *= alpha[u];
+      for (int u = 0; u < kU; ++u) l[u] = fall[u] > -126.0f ? l[u] * alpha[u] : rescale_sum(l[u], fall[u]);
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) {
         o[i][0] *= alpha[0];
         o[i][1] *= alpha[0];
         o[i][2] *= alpha[kSmall ? 0 : 1];
         o[i][3] *= alpha[kSmall ? 0 : 1];
+      }
+      if (low) {
+#pragma unroll
+        for (int s = 0; s < kTiles / 2; ++s)
+          if (inv[s] < 0.0f) {      // the same for the warp
+#pragma unroll
+            for (int u = 0; u < kU; ++u)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) l[u] += ex2_approx(x[2 * s + (e >> 1)][2 * u + (e & 1)] - (ref[u] + inv[s]));
+          }
       }
     }
     // weights, their sums, and O += W V
@@ -504,7 +517,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_s
       acc.y = __fmaf_rn(f, v.y, acc.y);
       acc.z = __fmaf_rn(f, v.z, acc.z);
       acc.w = __fmaf_rn(f, v.w, acc.w);
-      ll = __fmaf_rn(f, s_ml[(w * kOut + row) * 2 + 1], ll);
+      ll += rescale_sum(s_ml[(w * kOut + row) * 2 + 1], s_ml[(w * kOut + row) * 2] - rf);
     }
     if (splits == 1) {
       finish(row, d, acc, mm, ll);
@@ -545,7 +558,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks) attention_kv_s
         acc.y = __fmaf_rn(f, v[w].y, acc.y);
         acc.z = __fmaf_rn(f, v[w].z, acc.z);
         acc.w = __fmaf_rn(f, v[w].w, acc.w);
-        ll = __fmaf_rn(f, ml[w].y, ll);
+        ll += rescale_sum(ml[w].y, ml[w].x - rf);
       }
       finish(row, d, acc, mm, ll);
     }
@@ -599,7 +612,7 @@ __global__ void __launch_bounds__(128) attention_kv_join_kernel(const KvAttnPara
     if (s0 + lane < mine1) {
       const float2 ml = *reinterpret_cast<const float2*>(src + (s0 + lane) * step + D);
       f = ex2_approx(ml.x - ref);
-      l = __fmaf_rn(ml.y, f, l);
+      l += rescale_sum(ml.y, ml.x - ref);
     }
     const int end = min(32, mine1 - s0);
 #pragma unroll 8

@@ -180,6 +180,37 @@ __device__ __noinline__ float row_max(uint32_t taddr, uint32_t meta, float back)
   return top;
 }
 
+// A row's maximum with this block's, what O and l are scaled by for it (1: it has not moved), and l: scaled by the rest
+// where 2^(m - m') is below fp32's range.
+__device__ __noinline__ float4 look_row(uint32_t taddr, uint32_t meta, float back, float m, float l) {
+  const float m_new = fmaxf(m, row_max(taddr, meta, back));
+  const bool moved = m_new > m;
+  const float fall = moved ? fmaxf(m - m_new, -126.0f) : 0.0f;
+  return make_float4(m_new, ex2_approx(fall), moved ? rescale_sum(l, m - m_new - fall) : l, 0.0f);
+}
+
+// Adds to l the weights of keys of pages with a low scale, from their scores; a row without a maximum takes this block's.
+__device__ __noinline__ float2 low_sums(uint32_t taddr, uint32_t meta, float back, float m, float l) {
+  const float top = row_max(taddr, meta, back);
+  if (m == -INFINITY) m = top;
+  const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll 1
+  for (int h = 0; h < 2; ++h) {
+    float x[64];
+    tmem_ld_wait(taddr + 64 * h, x);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float4 f = meta_load(meta + 64 * h + 16 * u);
+      if (f.z < 0.0f) {       // the same for the warp
+        const float sc = score_scale(f.x, back);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) l += ex2_approx(__fmaf_rn(x[16 * u + k], sc, -ref));
+      }
+    }
+  }
+  return make_float2(m, l);
+}
+
 // Weights of half kHalf of a row's products, rounded to fp16 pairs; returns the
 // sum of weight / vs, and keeps in `most` a bound of the largest weight.
 template <int kHalf>
@@ -331,7 +362,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
   uint8_t* sq = smem;
   uint8_t* ring = sq + 2 * L::kTile;
   uint8_t* staged = ring + NS * L::kTile;                          // [converter warp][stage]
-  float4* s_meta = reinterpret_cast<float4*>(staged + kKtConvWarps * L::kStages * L::kUnit);      // [block % 16][16 keys]: x scale, log2 vs, 1/vs, page
+  float4* s_meta = reinterpret_cast<float4*>(staged + kKtConvWarps * L::kStages * L::kUnit);      // [block % 16][16 keys]: x scale, log2 vs, 1/vs or log2 vs, page
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_meta + kKtMeta * 8);
   uint64_t* q_full = bars;
   uint64_t* slot_full = bars + 1;
@@ -343,6 +374,8 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
   uint64_t* staged_full = meta_full + kKtMeta / kKtBatch;                     // [converter warp][stage]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(staged_full + kKtConvWarps * L::kStages);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert((1 + 2 * NS + 6 + kKtMeta / kKtBatch + kKtConvWarps * L::kStages) * 8 + 8 + kKtMeta / kKtBatch * 4 <= 384, "barriers' room");
+  uint32_t* s_low = tmem_slot + 2;         // [batch % 4]: whether keys are to be summed from their scores
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hk = blockIdx.y, b = blockIdx.z;
@@ -444,12 +477,16 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
     // first unit of batch m - 2.  (Each warp looking up its own units' took 1400 cycles a unit.)
     auto write_meta = [&](int m) {
       float4 f = make_float4(1.0f, -INFINITY, 0.0f, __int_as_float(-1));       // no page: weight 0
+      bool low = false;
       if (look_page >= 0) {   // a scale of zero: a page never written holds zeros
         const float v = fmaxf(look_v, kKvMinScale);
         const int poisoned = isnan(look_k) || isnan(look_v) ? kPoisoned : 0;
-        f = make_float4(fmaxf(look_k, kKvMinScale) * fabsf(p.scale_log2), log2f(v), __frcp_rn(v),
+        low = v < kKvLowScale && !poisoned;
+        f = make_float4(fmaxf(look_k, kKvMinScale) * fabsf(p.scale_log2), log2f(v), low ? log2f(v) : __frcp_rn(v),
                         __int_as_float(look_page | poisoned));
       }
+      const unsigned lows = __ballot_sync(0xffffffffu, low);
+      if (lane == 0) s_low[m % (kKtMeta / kKtBatch)] = lows;
       s_meta[(m * kKtBatch % kKtMeta) * 8 + lane] = f;
       __syncwarp();
       if (lane == 0) mbar_arrive(&meta_full[m % (kKtMeta / kKtBatch)]);
@@ -621,7 +658,11 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
       const int t = real ? full / p.group : 0, h = hk * p.group + (real ? full % p.group : 0);
       int first = 0, last = 0x7fffffff;                      // rows past the end never force masking
       if (real) kv_range(p, len, n_tok, t, first, last);
-      const int first_max = __reduce_max_sync(0xffffffffu, first), last_min = __reduce_min_sync(0xffffffffu, last);
+      // Blocks that need more than the usual are told by first_max alone, which a batch with low scales sets past every
+      // key: a condition of its own in the loop costs it 2 to 5 %.
+      constexpr int kLowBatch = 0x7fffffff;
+      int first_max = 0;
+      const int last_min = __reduce_min_sync(0xffffffffu, last);
       // Q rows to shared memory
       const uint32_t rows_at = smem_u32(sq + tile * L::kTile) + quad * 32 * 128;      // this warp's
       float back;
@@ -637,6 +678,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
       auto wait_meta = [&](int m) {
         ok = __all_sync(0xffffffffu, ok && mbar_wait_u32(smem_u32(&meta_full[m % (kKtMeta / kKtBatch)]),
                                                          (m / (kKtMeta / kKtBatch)) & 1, abort_flag));
+        first_max = *const_cast<volatile uint32_t*>(s_low + m % (kKtMeta / kKtBatch)) ? kLowBatch : __reduce_max_sync(0xffffffffu, first);
       };
       if (n_blocks > 0) wait_meta(0);
       for (int j = 0; j < n_blocks; ++j) {
@@ -647,7 +689,13 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
         // (after a wait that gave up the values mean nothing, but every warp keeps in step)
         tc_fence_after();
         const int key0 = (blk0 + j) * kKtKeys;
-        if (key0 < first_max || key0 + kKtKeys > last_min) mask_products(t_s, first - key0, last - key0);
+        if (key0 < first_max || key0 + kKtKeys > last_min) {
+          mask_products(t_s, first - key0, last - key0);
+          if (first_max == kLowBatch) {
+            const float2 ml = low_sums(t_s, meta, back, m, l);
+            m = ml.x, l = ml.y;
+          }
+        }
         // Against the maximum so far; only a row without one, or whose weights outgrow fp16's range by
         // their sums, looks for this block's.
         bool look = __any_sync(0xffffffffu, m == -INFINITY), moved = false;
@@ -655,10 +703,9 @@ __global__ void __launch_bounds__(kKtThreads, 1) attention_kv_tile_kernel(const 
         uint32_t w[64];
         while (true) {
           if (look) {
-            const float m_new = fmaxf(m, row_max(t_s, meta, back));
-            moved = m_new > m;
-            alpha = moved ? ex2_approx(m - m_new) : 1.0f;
-            m = m_new;
+            const float4 r = look_row(t_s, meta, back, m, l);
+            moved = r.x > m;
+            m = r.x, alpha = r.y, l = r.z;
           }
           const float ref = m == -INFINITY ? 0.0f : m;
           float most = 0.0f;

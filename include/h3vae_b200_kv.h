@@ -79,7 +79,8 @@ int h3b_kv_read_i8(const h3b_kv_cache* cache, const int32_t* page_table, int64_t
  *              (causal must be nonzero and window 0)
  *   lse        NULL, or fp32 [batch, q_heads, tokens]: the natural logarithm of each row's sum of exp
  * Rows that see no key (padding, an empty sequence, a position before the first key) are zero with lse
- * -infinity.  Keys a row does not see have no effect on it, whatever their page holds.
+ * -infinity.  Keys a row does not see have no effect on it, whatever their page holds.  Pages of zeros, or of values
+ * far below the others', count in the sum like any other beside values up to 2^77.
  * Workspace: h3b_attention_kv_i8_workspace_size(...) bytes of the same sizes, asked for with the same current
  * device (the plan goes by its number of SMs), 16-byte aligned; contents are not kept between calls.  Where that is
  * 16 the call needs none and takes NULL. */

@@ -158,3 +158,53 @@ def test_sequences_without_queries_are_not_looked_at(cuda_lib, t, group, wide):
     sel = torch.cat([pages[:1], every, pages[2:]]).contiguous()
     assert torch.equal(K.attention_kv_i8(q, cache, gone, _i32(lens), 0.125, selected=sel, **args), kept)
     assert _lib.device_error() == 0
+
+
+# ---------------------------------------------------------------------------
+# V scales far apart
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("t,group", [(1, 2), (6, 12), (130, 2)])
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("big", [1e4, 1e10, 1e18])
+@pytest.mark.parametrize("order", ["zeros first", "zeros last", "mixed"])
+@pytest.mark.parametrize("k_size", [1.0, 8.0])
+def test_value_pages_of_zeros_beside_large_ones(cuda_lib, t, group, wide, big, order, k_size):
+    """Keys whose values are zero count in the denominator like any other, however large the other pages' values are."""
+    from h3vae_b200 import kernels as K
+    rng = np.random.default_rng(60 + t)
+    lens, size = [500, 333], 32
+    ref, rows, table = _filled(rng, lens, 1, 64, size)
+    for row in rows:
+        pages = row[: len(row)]
+        zero = {"zeros first": pages[: len(pages) // 2], "zeros last": pages[len(pages) // 2:], "mixed": pages[::2]}[order]
+        for page in pages:
+            ref.scale["k"][page] *= np.float32(k_size)
+            ref.scale["v"][page] = R.TINY if page in zero else np.float32(ref.scale["v"][page] * big)
+        for page in zero:
+            ref.code["v"][page] = 0
+    cache = _cache(ref)
+    q = torch.from_numpy(rng.standard_normal((2, group, t, 64))).to(torch.bfloat16).cuda()
+    got, lse = K.attention_kv_i8(q, cache, _wide(table) if wide else table, _i32(lens), 0.125, return_lse=True)
+    out, want_lse, bound = _attend_all(ref, rows, q, lens, [t, t], 0.125, size)
+    R.check(got, out, bound, torch.bfloat16)
+    lse = lse.double().cpu().numpy()
+    assert np.abs(lse - want_lse).max() <= 2.0 ** -10
+
+
+@pytest.mark.parametrize("t", [1, 12, 130])
+def test_value_pages_of_zeros_in_parts_of_their_own(cuda_lib, t):
+    """The same where parts of the keys are joined: whole runs of zero pages beside runs of large values."""
+    from h3vae_b200 import kernels as K
+    rng = np.random.default_rng(61)
+    lens, size = [12000], 64
+    ref, rows, table = _filled(rng, lens, 1, 64, size)
+    ref.scale["v"][rows[0]] *= np.float32(1e12)
+    half = rows[0][: len(rows[0]) // 2]
+    ref.scale["v"][half] = R.TINY
+    ref.code["v"][half] = 0
+    cache = _cache(ref)
+    q = torch.from_numpy(rng.standard_normal((1, 1, t, 64))).to(torch.bfloat16).cuda()
+    sel = torch.arange(len(rows[0]), dtype=torch.int32, device="cuda").expand(1, 1, t, -1).contiguous()
+    out, _, bound = _attend_all(ref, rows, q, lens, [t], 0.125, size)
+    for tab, more in ((table, {}), (_wide(table), {}), (table, dict(selected=sel))):
+        R.check(K.attention_kv_i8(q, cache, tab, _i32(lens), 0.125, **more), out, bound, torch.bfloat16)
