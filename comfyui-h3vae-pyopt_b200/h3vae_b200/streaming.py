@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from . import kernels as K
-from .kv_cache import KVCacheI8
+from .kv_cache import PAGE_SIZES, KVCacheI8
 from .model import H3Decoder, rope_tables
 
 
@@ -28,6 +28,8 @@ class TokenStream:
             raise ValueError("TokenStream runs the INT8 block chain (H3Decoder(int8=True))")
         if batch < 1 or max_frames < 1 or min(grid_hw) < 1 or pages < 0:
             raise ValueError("batch, grid and max_frames must be positive, pages at least 0")
+        if page_size not in PAGE_SIZES:
+            raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
         cfg = decoder.cfg
         self.decoder, self.batch, self.pages = decoder, batch, pages
         self.per_frame = grid_hw[0] * grid_hw[1]
