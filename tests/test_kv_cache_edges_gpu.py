@@ -208,3 +208,26 @@ def test_value_pages_of_zeros_in_parts_of_their_own(cuda_lib, t):
     out, _, bound = _attend_all(ref, rows, q, lens, [t], 0.125, size)
     for tab, more in ((table, {}), (_wide(table), {}), (table, dict(selected=sel))):
         R.check(K.attention_kv_i8(q, cache, tab, _i32(lens), 0.125, **more), out, bound, torch.bfloat16)
+
+
+# ---------------------------------------------------------------------------
+# Selected pages for a frame of tokens
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,dim,group,t,lens,n", [("fp16", 64, 1, 192, [1500, 192], 7), ("bf16", 128, 3, 150, [900, 77], 4)])
+def test_selected_pages_for_a_frame(cuda_lib, dtype, dim, group, t, lens, n):
+    """Hundreds of tokens a call: every token's own choice, and attention over it."""
+    from h3vae_b200 import kernels as K
+    rng = np.random.default_rng(70 + t)
+    ref, rows, table = _filled(rng, lens, 2, dim, 64)
+    cache = _cache(ref)
+    q = torch.from_numpy(rng.standard_normal((2, 2 * group, t, dim))).to(TYPES[dtype]).cuda()
+    got = K.kv_select_i8(q, cache, table, _i32(lens), n)
+    qn = q.float().cpu().numpy()
+    for b, ln in enumerate(lens):
+        pos = [ln - t + i if ln - t + i >= 0 else -1 for i in range(t)]
+        for h in range(2):
+            want = R.select(qn[b, h * group: h * group + group], ref.scale["k"][rows[b], h], ref.k_sum[rows[b], h], pos,
+                            n, 64, group)
+            assert np.array_equal(got[b, h].cpu().numpy(), want), (b, h)
+    out, _, bound = _attend_all(ref, rows, q, lens, [t, t], dim ** -0.5, 64, selected=got.cpu().numpy())
+    R.check(K.attention_kv_i8(q, cache, table, _i32(lens), dim ** -0.5, selected=got), out, bound, TYPES[dtype])
