@@ -12,7 +12,8 @@ namespace {
 // 33 rows 20 / 16, 64 rows 20 / 19; 8 x 8 heads over 8192 keys, dim 128, fp16 and
 // bf16: 17 rows 80 / 81 and 72, 33 rows 80 / 112 and 99, 64 rows 81 / 144 and 128; 32 x
 // 16 heads over 2000 keys: 40 rows 127 / 103, 70 rows 128 / 163; 2 x 16 heads over 1024 keys:
-// 64 rows (17 MB) 17 / 12, 128 rows (34 MB) 18 / 33.
+// 64 rows (17 MB) 17 / 12, 128 rows (34 MB) 18 / 33.  One limit for both dims: at dim 128
+// and 17 to 48 rows over long caches it takes the slower side, by up to 40 % (33 rows, fp16).
 constexpr int64_t kTileRows = 48;
 constexpr int64_t kTileBytes = int64_t(24) << 20;
 
@@ -51,9 +52,9 @@ KvPlan kv_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t tokens,
   const int64_t items = batch * kv_heads * k.row_tiles * (n_selected > 0 ? tokens : 1);
   const int64_t tiles = ((n_selected > 0 ? n_selected : width) * page + keys - 1) / keys;
   // Up to eight runs of a row tile's keys join inside a cluster: one launch and no trip through global memory
-  // (one token over 1797 keys, 16 heads: 6.5 us, 8.6 with a second kernel).  For short runs, and for selected pages,
+  // (one token over 1797 keys, 16 heads: 7.2 us, about 2 more with a second kernel).  For short runs, and for selected pages,
   // which are as many for every row; long sequences of different lengths are better cut into equal parts
-  // (16 x 6553..32768 keys: 154 us in clusters of eight, 129 in parts).
+  // (16 x 6553..32768 keys: 154 us in clusters of eight, 129 in parts; 134 with low scales looked for).
   const int64_t wave = kSplitBlocks * h3b_host::num_sms();
   const int64_t c = std::max<int64_t>(
       1, std::min({(int64_t)kSplitCluster, wave / items, (tiles + kSplitWarps - 1) / kSplitWarps}));

@@ -97,8 +97,9 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 }
 
 // A query row as fp16.  bf16 rows are scaled by a power of two so that their
-// largest value lies in [1, 2): every value that matters at fp32 precision of
-// the product is then exact in fp16; `back` undoes the scaling.
+// largest value lies in [1, 2).  Values down to 2^-17 of it (8 bits each) are then
+// exact in fp16, and smaller ones are off by 2^-25 of it at most, half an fp32 ulp
+// of the largest; `back` undoes the scaling.
 __device__ __forceinline__ float row_scaling(__half, float, float& back) {
   back = 1.0f;
   return 1.0f;

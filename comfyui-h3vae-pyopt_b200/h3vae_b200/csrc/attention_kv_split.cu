@@ -29,12 +29,15 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
 // bf16 outputs round eight times coarser and go without.
 //
 // The rows see nearly all keys of their sequence, so a call moves the cache's
-// bytes once and is bound by HBM when it is long and by latency (table, scale
+// bytes once per 16-row tile (with selected pages, a token's pages once per token and
+// tile) and is bound by HBM when it is long and by latency (table, scale
 // and code loads in a row, then the join) when it is short.  One token each over
-// 16 x 6553..32768 keys, 8 heads of dim 128, 32 query heads: 690 MB in 129 us =
-// 5.3 TB/s, with the issue slots 52 % and the tensor pipe 34 % in use; 12 warps an
+// 16 x 6553..32768 keys, 8 heads of dim 128, 32 query heads: 690 MB in 134 us =
+// 5.2 TB/s, with the issue slots 51 % and the tensor pipe 33 % in use; 12 warps an
 // SM hide each other's latency.  Before runs were fitted to waves, at 141 us: 8 warps
-// 154 us, tiles of half the size 165 us, of twice the size 178 us.  One token over 1797 keys of 16 heads: 6.5 us.
+// 154 us, tiles of half the size 165 us, of twice the size 178 us.  One token over 1797 keys of 16 heads: 7.2 us.
+// (Pages with a low scale of V cost their branch and the two-step joins: 131 and 7.0 us without;
+// a second instance of the loop for them spills: 137 us.)
 constexpr int kSplitWarps = 4;
 constexpr int kSplitStages = 2;
 constexpr int kSplitBlocks = 3;       // blocks an SM holds (two with three stages: 154 against 141 us on 16 x 6553..32768 keys)

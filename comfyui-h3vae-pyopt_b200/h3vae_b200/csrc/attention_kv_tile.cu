@@ -24,12 +24,17 @@
 // the block redone and O rescaled in TMEM.  Blocks that no row of the CTA sees are
 // not visited, and only blocks on an edge of a row's range mask keys.
 //
+// Weights have 11 bits and no low part (the second operand of the few-row kernel): rows see hundreds of
+// keys here, their roundings average out, and the product would be taken twice.  Error against 64 bits,
+// with the weights in fp32 beside it: 1024 tokens over 5120 keys, fp16, 2.02e-4 and 1.97e-4; the causal
+// prompt, bf16, 1.639e-3 and 1.638e-3.
+//
 // What bounds it: not the tensor pipe (27 % active at dim 64) nor the SFU (16
 // exponentials a clock: 55 %), but the chain of a row tile -- products, wait, weights
 // (2000 to 2200 cycles a block), wait, products -- which two row tiles only half cover,
 // and at dim 128 the converters beside it.  1024 tokens over 5120 keys, 2 x 16 heads of
-// dim 64: 84 us = 510 TFLOP/s; a causal prompt of 8101 tokens, 2 x 32 heads over 8 of dim
-// 128: 1.16 ms = 927 TFLOP/s.  A call over 256 keys takes 12 us at dim 64 and 17 at dim
+// dim 64: 81 us = 530 TFLOP/s (bf16 84); a causal prompt of 8101 tokens, 2 x 32 heads over 8 of
+// dim 128: 1.20 ms = 897 TFLOP/s (1.17 without pages of a low scale; 81 and 82 at dim 64).  A call over 256 keys takes 12 us at dim 64 and 17 at dim
 // 128, every further 128 keys 2.0 and 2.3.  Measured and left, against 85 us and 1.27 ms:
 // 64-key steps with two buffers of products (99 us, 1.45 ms: twice the waits of the
 // issuing warp), 16 warps with an issuer per row tile and six converters (91 us, 1.52 ms:

@@ -11,7 +11,9 @@
 // Two steps: scores (a thread per page, all rows of the sequence and head
 // from shared memory) and the selection (a block per row: the (n-1)-th largest
 // key by bisection, then an ordered compaction); a kernel each, or one for few tokens.
-// Both are latency: 2048 pages of 16 heads, 4 MB of sums, take 10 us together (3.6 for the scores alone).
+// Both are latency: 2048 pages of 16 heads, 4 MB of sums, take 11 us together (3.6 for the scores alone).
+// Tokens are not spread over blocks: a block of the score kernel takes them one after the other, which is made for few
+// (1024 tokens x 4 x 16 heads: 480 us over 80 pages, 784 us over 640).
 #include <algorithm>
 
 #include "kv_common.cuh"

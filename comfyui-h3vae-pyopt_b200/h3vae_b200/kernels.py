@@ -19,7 +19,8 @@ F16 = torch.float16
 I8 = torch.int8
 F32 = torch.float32
 
-# Kernel-launch accounting (bench.py reads it): number of library kernels each wrapper launches.
+# Kernel-launch accounting (bench.py reads it): number of library kernels each wrapper launches (the cache's calls, which
+# launch one or two by a plan of the library's, count one).
 LAUNCHES = {"count": 0}
 # Optional per-call CUDA-event timing of the INT8 conv (bench.py's live roofline measurement):
 # when CONV_TIMING is a list, conv3d_i8 appends (start_event, end_event, int8_ops) per launch.
